@@ -1,0 +1,534 @@
+// Block-scaled 8-bit copies of activations and weights: fp32 / fp16 / bf16 -> e4m3 values with a power-of-two scale for each
+// block of 1 x 128 or 128 x 128, and back; and the two-bit checkpoint of the (Jump)ReLU.
+//
+// The scale of a block is the smallest power of two s (at least 2^-126) with amax / s <= 448, amax over the block's finite values;
+// 1 where all are zero.  With a power of two the quotient x / s and the product q * s are exact, so that the only rounding is the
+// one to e4m3 (half a step: 2^-4 of the value), whichever way a copy was made, and a copy of a copy is the copy.  e4m3 has no
+// infinity: what is not finite becomes NaN, and does not count for the scale.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "../../include/clt_b200.h"
+#include "common.cuh"
+#include "kernels.h"
+
+using namespace clt;
+
+namespace {
+
+// ---- 8 consecutive values ----------------------------------------------------------------------
+template <class T>
+struct Vec8;
+template <>
+struct Vec8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
+  }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+  }
+  __device__ __forceinline__ void put(const float (&v)[8]) {
+    a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  __device__ __forceinline__ void store(float* p) const { st_cs8(p, a, b); }
+};
+template <class T>
+struct Vec8Half {
+  uint4 a;
+  __device__ __forceinline__ void load(const T* p) { a = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), a); }
+};
+template <>
+struct Vec8<__nv_bfloat16> : Vec8Half<__nv_bfloat16> {
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[2 * i] = __uint_as_float(w[i] << 16), o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  __device__ __forceinline__ void put(const float (&v)[8]) {
+    a = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+};
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+struct Vec8<__half> : Vec8Half<__half> {
+  __device__ __forceinline__ void get(float (&o)[8]) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[2 * i] = f.x, o[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void put(const float (&v)[8]) {
+    a = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+  }
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f32(float& o, float v) { o = v; }
+__device__ __forceinline__ void from_f32(__half& o, float v) { o = __float2half_rn(v); }
+__device__ __forceinline__ void from_f32(__nv_bfloat16& o, float v) { o = __float2bfloat16_rn(v); }
+
+// `n` of 8 values (the rest 0); `vec`: a 16-byte aligned address and all 8 there
+template <class T>
+__device__ __forceinline__ Vec8<T> load8(const T* p, int n, bool vec) {
+  Vec8<T> r;
+  if (vec) {
+    r.load(p);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    r.put(v);
+  }
+  return r;
+}
+template <class T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+  if (vec) {
+    Vec8<T> r;
+    r.put(v);
+    r.store(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) from_f32(p[i], v[i]);
+  }
+}
+
+// ---- scale and rounding ----------------------------------------------------------------------------
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a <= 3.402823466e38f ? a : 0.f;  // 0 for infinities and NaN
+}
+// amax = m 2^e with m in [1, 2), and 448 = 1.75 * 2^8: 2^(e-8), or 2^(e-7) where m > 1.75.  (A subnormal amax has e = -127
+// here, its scale is the least one either way.)
+__device__ __forceinline__ float block_scale(float amax) {
+  if (amax == 0.f) return 1.f;
+  const uint32_t u = __float_as_uint(amax);
+  int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < -126 ? -126 : e;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// 1 / 2^e; exact for every scale (2^-126 .. 2^120)
+__device__ __forceinline__ float inverse_scale(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
+
+__device__ __forceinline__ float not_inf(float v) { return fabsf(v) <= 3.402823466e38f ? v : __uint_as_float(0x7fffffffu); }
+
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv) {
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(not_inf(v[2 * i]) * inv, not_inf(v[2 * i + 1]) * inv), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+
+__device__ __forceinline__ float max16(float v) {  // over groups of 16 lanes
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+struct Source {
+  const void* x;
+  long long ld, z;  // elements
+  int R, C;
+  int vec;  // rows start on 16 bytes
+};
+
+// One CTA per 128 x 128 block, 16 lanes x 8 values to a row, 8 rows to a thread: the block is read once, all of it at a time.
+// sums (may be NULL): sums[z, block of rows, c] = the block's column sums (of what came in), for bias gradients.
+template <class T>
+__global__ void __launch_bounds__(256) quantize_tile_kernel(Source s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
+                                                            float* __restrict__ sums, int row_blocks, int col_blocks) {
+  __shared__ float part[8];
+  __shared__ float colsum[16][128];
+  const int cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks, z = blockIdx.y;
+  const int g = threadIdx.x >> 4, c = cb * 128 + (threadIdx.x & 15) * 8;
+  const int n = s.C - c;
+  const bool vec = s.vec && n >= 8;
+  const T* x = (const T*)s.x + z * s.z + (long long)(rb * 128 + g) * s.ld + c;
+  const int rows = s.R - rb * 128 - g;
+  Vec8<T> v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = load8<T>(x + (long long)(16 * i) * s.ld, 16 * i < rows ? n : 0, vec && 16 * i < rows);
+  float amax = 0.f, f[8];
+  float cs[8] = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i].get(f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, finite_abs(f[k]));
+    if (sums != nullptr) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) cs[k] += f[k];
+    }
+  }
+  amax = max16(amax);
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+  if (sums != nullptr) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) colsum[g][(threadIdx.x & 15) * 8 + k] = cs[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, part[i]);
+  const float scale = block_scale(amax), inv = inverse_scale(scale);
+  if (threadIdx.x == 0) scales[((long long)z * row_blocks + rb) * col_blocks + cb] = scale;
+  uint8_t* out = q + ((long long)z * s.R + rb * 128 + g) * q_ld + c;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (16 * i < rows && c < q_ld) {
+      v[i].get(f);
+      *reinterpret_cast<uint2*>(out + (long long)(16 * i) * q_ld) = to_e4m3x8(f, inv);
+    }
+  }
+  if (sums != nullptr && threadIdx.x < 128 && cb * 128 + threadIdx.x < s.C) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += colsum[i][threadIdx.x];
+    sums[((long long)z * row_blocks + rb) * s.C + cb * 128 + threadIdx.x] = t;
+  }
+}
+
+// 1 x 128 blocks: 16 lanes to a block, kAhead blocks in flight per group of lanes.
+constexpr int kAhead = 4;
+template <class T>
+__global__ void __launch_bounds__(256) quantize_row_kernel(Source s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
+                                                           int col_blocks, long long blocks) {
+  const int lane = threadIdx.x & 15;
+  const long long first = ((long long)blockIdx.x * 16 + (threadIdx.x >> 4)) * kAhead;
+  Vec8<T> v[kAhead];
+  long long row[kAhead];
+  int c[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const long long b = first + i;
+    row[i] = b / col_blocks;
+    c[i] = (int)(b - row[i] * col_blocks) * 128 + lane * 8;
+    const long long z = row[i] / s.R, r = row[i] - z * s.R;
+    const int n = b < blocks ? s.C - c[i] : 0;
+    v[i] = load8<T>((const T*)s.x + z * s.z + r * s.ld + c[i], n, s.vec && n >= 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    float f[8], amax = 0.f;
+    v[i].get(f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, finite_abs(f[k]));
+    const float scale = block_scale(max16(amax));
+    if (first + i < blocks) {
+      if (lane == 0) scales[first + i] = scale;
+      if (c[i] < q_ld) *reinterpret_cast<uint2*>(q + row[i] * q_ld + c[i]) = to_e4m3x8(f, inverse_scale(scale));
+    }
+  }
+}
+
+struct ScaleMap {
+  const float* p;
+  long long z, r, c;
+  int shift;
+};
+
+// 16 values of a row to a thread.
+template <class T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ q, long long q_ld, long long q_z, ScaleMap sc,
+                                                         T* __restrict__ out, int R, int C, int groups, long long n, int q_vec,
+                                                         int out_vec) {
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= n) return;
+  const long long row = i / groups;
+  const int c = (int)(i - row * groups) * 16;
+  const long long z = row / R, r = row - z * R;
+  const uint8_t* p = q + z * q_z + r * q_ld + c;
+  const int left = C - c;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (q_vec && left >= 16) {
+    const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
+    w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (k < left) w[k >> 2] |= (uint32_t)p[k] << 8 * (k & 3);
+  }
+  const float s = __ldg(sc.p + z * sc.z + (r >> sc.shift) * sc.r + (c >> 7) * sc.c);
+  T* o = out + row * C + c;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t two = (w[2 * h + (k >> 1)] >> 16 * (k & 1)) & 0xffff;
+      const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+      f[2 * k] = t.x * s, f[2 * k + 1] = t.y * s;
+    }
+    store8<T>(o + 8 * h, left - 8 * h, out_vec && left >= 8 * h + 8, f);
+  }
+}
+
+struct Bandwidth {
+  const float* p;  // on the device, or NULL for
+  float value;
+  __device__ __forceinline__ float get() const { return p != nullptr ? __ldg(p) : value; }
+};
+
+// out[z, c] = sum over the chunks, in their order, of part[z, chunk, c]; times -(theta / bandwidth) where theta is given.
+__global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict__ part, float* __restrict__ out, int chunks, int C,
+                                                         const float* __restrict__ theta, Bandwidth bandwidth) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= C) return;
+  const float* p = part + (long long)blockIdx.y * chunks * C + c;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < chunks; ++i) acc += __ldcs(p + (long long)i * C);
+  if (theta != nullptr) acc *= -(theta[c] / bandwidth.get());
+  out[(long long)blockIdx.y * C + c] = acc;
+}
+
+// ---- (Jump)ReLU with a two-bit checkpoint ---------------------------------------------------------------
+// A thread has 8 columns with their thresholds and walks down the rows, two of them in flight.  A word of the checkpoint is 16 bits for 8
+// values: the low byte has bit i where the gradient passes (x >= 0; ReLU: x > 0), the high byte where theta - bw/2 < x <= theta + bw/2,
+// the window in which the threshold gets a gradient.  Both bounds are rounded down from 64 bits, which decides the comparisons with
+// an fp32 x as the exact bounds would.
+struct Window {
+  float lo[8], hi[8], theta[8];
+};
+__device__ __forceinline__ void load_window(Window& w, const float* theta, Bandwidth bandwidth, int c, int n) {
+  const double half = 0.5 * (double)bandwidth.get();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float t = k < n ? theta[c + k] : 0.f;
+    w.theta[k] = t;
+    w.lo[k] = __double2float_rd((double)t - half);
+    w.hi[k] = __double2float_rd((double)t + half);
+  }
+}
+
+template <class T, bool kJump>
+__global__ void __launch_bounds__(256) jump_relu_fwd_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ theta,
+                                                            Bandwidth bandwidth, T* __restrict__ y,
+                                                            uint16_t* __restrict__ bits, int R, int C, int rows_per_cta, int in_vec,
+                                                            int out_vec) {
+  const int words = (C + 7) / 8, w = blockIdx.x * 256 + threadIdx.x;
+  if (w >= words) return;
+  const int c = w * 8, n = C - c;
+  Window win;
+  if constexpr (kJump) load_window(win, theta, bandwidth, c, n);
+  const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
+  const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
+#pragma unroll 2
+  for (int r = r0; r < r1; ++r) {
+    const Vec8<T> v = load8<T>(x + r * ld + c, n, iv);
+    float f[8];
+    v.get(f);
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float t = f[k];
+      if constexpr (kJump) {
+        m |= (t < 0.f ? 0u : 1u) << k;
+        m |= (t > win.lo[k] && t <= win.hi[k] ? 256u : 0u) << k;
+        f[k] = (t <= win.theta[k] || t <= 0.f) ? 0.f : t;  // NaN stays
+      } else {
+        m |= (t <= 0.f ? 0u : 1u) << k;
+        f[k] = t <= 0.f ? 0.f : t;
+      }
+    }
+    store8<T>(y + (long long)r * C + c, n, ov, f);
+    bits[(long long)r * words + w] = (uint16_t)m;
+  }
+}
+
+template <class T, bool kJump>
+__global__ void __launch_bounds__(256) jump_relu_bwd_kernel(const T* __restrict__ g, long long ld, const uint16_t* __restrict__ bits,
+                                                            T* __restrict__ dx, float* __restrict__ part, int R, int C,
+                                                            int rows_per_cta, int in_vec, int out_vec) {
+  const int words = (C + 7) / 8, w = blockIdx.x * 256 + threadIdx.x;
+  if (w >= words) return;
+  const int c = w * 8, n = C - c;
+  const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
+  const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
+  float acc[8] = {};
+#pragma unroll 4
+  for (int r = r0; r < r1; ++r) {
+    const Vec8<T> v = load8<T>(g + r * ld + c, n, iv);
+    const uint32_t m = bits[(long long)r * words + w];
+    float f[8];
+    v.get(f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (kJump && (m >> (8 + k) & 1)) acc[k] += f[k];
+      if (!(m >> k & 1)) f[k] = 0.f;
+    }
+    store8<T>(dx + (long long)r * C + c, n, ov, f);
+  }
+  if constexpr (kJump) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) part[(long long)blockIdx.y * C + c + k] = acc[k];
+  }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+long long up(long long a, long long b) { return (a + b - 1) / b; }
+int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+
+// Rows that one CTA of the (Jump)ReLU kernels walks: enough CTAs for the chip, at least 8 rows (a thread's thresholds are read once).
+int rows_per_cta(int R, int C, int sms) {
+  const long long across = up(up(C, 8), 256), want = up(8ll * sms, across);
+  long long rows = up(R, want);
+  return (int)(rows < 8 ? 8 : rows > 128 ? 128 : rows);
+}
+
+template <class T>
+int quantize(const Source& s, uint8_t* q, int q_ld, float* scales, float* sums, int Z, int block_rows, cudaStream_t st) {
+  const int cb = (int)up(s.C, 128);
+  if (block_rows == 1) {
+    const long long blocks = (long long)Z * s.R * cb, grid = up(blocks, 16 * kAhead);
+    CLT_CHECK_ARG(grid < (1ll << 31), "fp8_quantize: too many blocks");
+    quantize_row_kernel<T><<<(unsigned)grid, 256, 0, st>>>(s, q, q_ld, scales, cb, blocks);
+  } else {
+    const long long rb = up(s.R, 128);
+    CLT_CHECK_ARG(rb * cb < (1ll << 31) && Z <= 65535, "fp8_quantize: too many blocks");
+    quantize_tile_kernel<T><<<dim3((unsigned)(rb * cb), Z), 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
+  }
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+template <class T>
+int dequantize(const uint8_t* q, long long q_ld, long long q_z, const ScaleMap& sc, T* out, int Z, int R, int C, cudaStream_t st) {
+  const int groups = (int)up(C, 16);
+  const long long n = (long long)Z * R * groups, grid = up(n, 256);
+  CLT_CHECK_ARG(grid < (1ll << 31), "fp8_dequantize: too many values");
+  dequantize_kernel<T><<<(unsigned)grid, 256, 0, st>>>(q, q_ld, q_z, sc, out, R, C, groups, n,
+                                                       aligned16(q) && q_ld % 16 == 0 && (Z == 1 || q_z % 16 == 0),
+                                                       aligned16(out) && (long long)C * sizeof(T) % 16 == 0);
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+template <class T>
+int jump_fwd(const T* x, long long ld, const float* theta, Bandwidth bw, T* y, uint16_t* bits, int R, int C, int sms,
+             cudaStream_t st) {
+  const int rows = rows_per_cta(R, C, sms);
+  const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
+  const int iv = aligned16(x) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(y) && C * (long long)sizeof(T) % 16 == 0;
+  if (theta != nullptr)
+    jump_relu_fwd_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
+  else
+    jump_relu_fwd_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+template <class T>
+int jump_bwd(const T* g, long long ld, const uint16_t* bits, const float* theta, Bandwidth bw, T* dx, float* dtheta, float* ws,
+             int R, int C, int sms, cudaStream_t st) {
+  const int rows = rows_per_cta(R, C, sms);
+  const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
+  const int iv = aligned16(g) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(dx) && C * (long long)sizeof(T) % 16 == 0;
+  if (theta != nullptr) {
+    jump_relu_bwd_kernel<T, true><<<grid, 256, 0, st>>>(g, ld, bits, dx, ws, R, C, rows, iv, ov);
+    sum_chunks_kernel<<<dim3((unsigned)up(C, 256), 1), 256, 0, st>>>(ws, dtheta, (int)grid.y, C, theta, bw);
+  } else {
+    jump_relu_bwd_kernel<T, false><<<grid, 256, 0, st>>>(g, ld, bits, dx, nullptr, R, C, rows, iv, ov);
+  }
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int clt_fp8_quantize(const void* x, int in_dtype, int64_t ld, int64_t z_stride, void* q, int64_t q_ld, float* scales,
+                     float* column_sums, int Z, int R, int C, int block_rows, clt_stream_t stream) {
+  CLT_CHECK_ARG(x && q && scales, "fp8_quantize: null pointer");
+  CLT_CHECK_ARG(Z > 0 && R > 0 && C > 0, "fp8_quantize: bad dims Z=%d R=%d C=%d", Z, R, C);
+  CLT_CHECK_ARG(in_dtype >= 0 && in_dtype <= 2, "fp8_quantize: input type %d", in_dtype);
+  CLT_CHECK_ARG(block_rows == 1 || block_rows == 128, "fp8_quantize: blocks of %d rows (1 or 128)", block_rows);
+  CLT_CHECK_ARG(column_sums == nullptr || block_rows == 128, "fp8_quantize: column sums come with blocks of 128 rows");
+  CLT_CHECK_ARG(q_ld >= C && q_ld % 16 == 0 && q_ld < (1ll << 31) && aligned16(q),
+                "fp8_quantize: rows of the copy must be 16-byte aligned (distance %lld)", (long long)q_ld);
+  const int e = elem_size(in_dtype);
+  CLT_CHECK_ARG((uintptr_t)x % e == 0, "fp8_quantize: misaligned input");
+  const Source s{x, ld, z_stride, R, C, aligned16(x) && ld * e % 16 == 0 && (Z == 1 || z_stride * e % 16 == 0)};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (in_dtype == 0) return quantize<float>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
+  if (in_dtype == 1) return quantize<__half>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
+  return quantize<__nv_bfloat16>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
+}
+
+int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,
+                       int block_rows, void* out, int out_dtype, int Z, int R, int C, clt_stream_t stream) {
+  CLT_CHECK_ARG(q && scales && out, "fp8_dequantize: null pointer");
+  CLT_CHECK_ARG(Z > 0 && R > 0 && C > 0, "fp8_dequantize: bad dims Z=%d R=%d C=%d", Z, R, C);
+  CLT_CHECK_ARG(out_dtype >= 0 && out_dtype <= 2, "fp8_dequantize: output type %d", out_dtype);
+  CLT_CHECK_ARG(block_rows == 1 || block_rows == 128, "fp8_dequantize: blocks of %d rows (1 or 128)", block_rows);
+  CLT_CHECK_ARG((uintptr_t)out % elem_size(out_dtype) == 0, "fp8_dequantize: misaligned output");
+  const ScaleMap sc{scales, s_z, s_r, s_c, block_rows == 1 ? 0 : 7};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (out_dtype == 0) return dequantize<float>((const uint8_t*)q, q_ld, q_z, sc, (float*)out, Z, R, C, st);
+  if (out_dtype == 1) return dequantize<__half>((const uint8_t*)q, q_ld, q_z, sc, (__half*)out, Z, R, C, st);
+  return dequantize<__nv_bfloat16>((const uint8_t*)q, q_ld, q_z, sc, (__nv_bfloat16*)out, Z, R, C, st);
+}
+
+int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_stream_t stream) {
+  CLT_CHECK_ARG(part && out, "sum_chunks: null pointer");
+  CLT_CHECK_ARG(Z > 0 && Z <= 65535 && chunks >= 0 && C > 0, "sum_chunks: bad dims Z=%d chunks=%d C=%d", Z, chunks, C);
+  sum_chunks_kernel<<<dim3((unsigned)up(C, 256), Z), 256, 0, (cudaStream_t)stream>>>(part, out, chunks, C, nullptr,
+                                                                                          Bandwidth{nullptr, 1.f});
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+int clt_jump_relu_chunks(int R, int C) { return R > 0 && C > 0 ? (int)up(R, rows_per_cta(R, C, device_sm_count())) : 0; }
+
+int clt_jump_relu_fwd(const void* x, int64_t ld, const float* theta, const float* bandwidth, float bandwidth_value, void* y,
+                      void* bits, int dtype, int R, int C, clt_stream_t stream) {
+  CLT_CHECK_ARG(x && y && bits, "jump_relu_fwd: null pointer");
+  CLT_CHECK_ARG(theta == nullptr || bandwidth != nullptr || bandwidth_value > 0.f, "jump_relu_fwd: bandwidth must be positive");
+  CLT_CHECK_ARG(R > 0 && C > 0 && C <= (1 << 30) && ld >= 0, "jump_relu_fwd: bad dims R=%d C=%d", R, C);
+  CLT_CHECK_ARG(dtype >= 0 && dtype <= 2 && (uintptr_t)x % elem_size(dtype) == 0 && (uintptr_t)y % elem_size(dtype) == 0,
+                "jump_relu_fwd: type %d or misaligned pointer", dtype);
+  const int sms = device_sm_count();
+  CLT_CHECK_ARG(up(R, rows_per_cta(R, C, sms)) <= 65535, "jump_relu_fwd: too many rows");
+  cudaStream_t st = (cudaStream_t)stream;
+  uint16_t* b = (uint16_t*)bits;
+  const Bandwidth bw{bandwidth, bandwidth_value};
+  if (dtype == 0) return jump_fwd<float>((const float*)x, ld, theta, bw, (float*)y, b, R, C, sms, st);
+  if (dtype == 1) return jump_fwd<__half>((const __half*)x, ld, theta, bw, (__half*)y, b, R, C, sms, st);
+  return jump_fwd<__nv_bfloat16>((const __nv_bfloat16*)x, ld, theta, bw, (__nv_bfloat16*)y, b, R, C, sms, st);
+}
+
+int clt_jump_relu_bwd(const void* g, int64_t ld, const void* bits, const float* theta, const float* bandwidth,
+                      float bandwidth_value, void* dx, float* dtheta, float* ws, int64_t ws_floats, int dtype, int R, int C,
+                      clt_stream_t stream) {
+  CLT_CHECK_ARG(g && bits && dx && (theta == nullptr || (dtheta && ws)), "jump_relu_bwd: null pointer");
+  CLT_CHECK_ARG(theta == nullptr || bandwidth != nullptr || bandwidth_value > 0.f, "jump_relu_bwd: bandwidth must be positive");
+  CLT_CHECK_ARG(R > 0 && C > 0 && C <= (1 << 30) && ld >= 0, "jump_relu_bwd: bad dims R=%d C=%d", R, C);
+  CLT_CHECK_ARG(dtype >= 0 && dtype <= 2 && (uintptr_t)g % elem_size(dtype) == 0 && (uintptr_t)dx % elem_size(dtype) == 0,
+                "jump_relu_bwd: type %d or misaligned pointer", dtype);
+  const int sms = device_sm_count();
+  const long long chunks = up(R, rows_per_cta(R, C, sms));
+  CLT_CHECK_ARG(chunks <= 65535, "jump_relu_bwd: too many rows");
+  CLT_CHECK_ARG(theta == nullptr || chunks * C <= ws_floats, "jump_relu_bwd: %lld floats of scratch, %lld needed",
+                (long long)ws_floats, chunks * C);
+  cudaStream_t st = (cudaStream_t)stream;
+  const uint16_t* b = (const uint16_t*)bits;
+  const Bandwidth bw{bandwidth, bandwidth_value};
+  if (dtype == 0) return jump_bwd<float>((const float*)g, ld, b, theta, bw, (float*)dx, dtheta, ws, R, C, sms, st);
+  if (dtype == 1) return jump_bwd<__half>((const __half*)g, ld, b, theta, bw, (__half*)dx, dtheta, ws, R, C, sms, st);
+  return jump_bwd<__nv_bfloat16>((const __nv_bfloat16*)g, ld, b, theta, bw, (__nv_bfloat16*)dx, dtheta, ws, R, C, sms, st);
+}
+
+}  // extern "C"

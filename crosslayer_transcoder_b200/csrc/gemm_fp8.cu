@@ -1,0 +1,181 @@
+// C entry points of the 8-bit contraction: geometry, operand descriptions, parts of long contractions.
+#include "../../include/clt_b200.h"
+#include "gemm_fp8.cuh"
+#include "kernels.h"
+
+using namespace clt;
+
+namespace {
+
+inline long long up(long long a, long long b) { return (a + b - 1) / b; }
+
+// Pairs of CTAs where rounding the rows up to 256 adds at most an eighth and pairs fill half the chip.
+bool use_pair(const GemmGeom& g, int sms) {
+  const long long n_tiles = up(g.N, f8::kBN), single = up(g.M, 128) * n_tiles * g.nz, pairs = up(g.M, 256) * n_tiles * g.nz;
+  return pairs >= sms / 2 && pairs * 16 <= single * 9;
+}
+
+// Cuts the contraction into parts (gemm.cuh) where there are fewer output tiles than SMs, or chains so uneven that the longest
+// outlasts a fair share by half; sets g.kb_per_part and returns the number of parts, or 0 for whole chains.
+int plan_parts(GemmGeom& g, int sms) {
+  const int kb_per_seg = (int)up(g.Kseg, f8::kBK);
+  const long long tiles = up(g.M, 128) * up(g.N, f8::kBN);
+  long long total = 0, longest = 0;
+  for (int z = 0; z < g.nz; ++z) {
+    const long long n = (long long)seg_count(g, z) * kb_per_seg;
+    total += n;
+    longest = n > longest ? n : longest;
+  }
+  g.kb_per_part = 0;
+  if (longest < 8 || longest * sms * 2 <= total * tiles * 3) return 0;
+  const long long share = up(total * tiles, sms), part = share < 4 ? 4 : share;
+  g.kb_per_part = (int)part;
+  long long parts = 0;
+  for (int z = 0; z < g.nz; ++z) parts += part_count(g, z, kb_per_seg);
+  if (parts <= g.nz || parts > 65535) return g.kb_per_part = 0;
+  return (int)parts;
+}
+
+template <class T>
+struct FromFloat;
+template <>
+struct FromFloat<float> {
+  __device__ static float get(float v) { return v; }
+};
+template <>
+struct FromFloat<__half> {
+  __device__ static __half get(float v) { return __float2half_rn(v); }
+};
+template <>
+struct FromFloat<__nv_bfloat16> {
+  __device__ static __nv_bfloat16 get(float v) { return __float2bfloat16_rn(v); }
+};
+
+// out[z, m, n] = bias[z, n] + the partial sums of z's parts, in their order.
+template <class T>
+__global__ void __launch_bounds__(256) fp8_sum_parts_kernel(const float* __restrict__ ws, f8::Out out, GemmGeom g, int kb_per_seg) {
+  const int z = blockIdx.y;
+  const long long slab = (long long)g.M * g.N, i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= slab) return;
+  int first = 0;
+  for (int u = 0; u < z; ++u) first += part_count(g, u, kb_per_seg);
+  const int parts = part_count(g, z, kb_per_seg);
+  const long long m = i / g.N;
+  const int n = (int)(i - m * g.N);
+  const float* p = ws + first * slab + i;
+  float acc = out.bias != nullptr ? __ldg(out.bias + z * out.bias_z + n) : 0.f;
+#pragma unroll 8
+  for (int j = 0; j < parts; ++j) acc += __ldcs(p + j * slab);
+  ((T*)out.p)[z * out.z + m * out.ld + n] = FromFloat<T>::get(acc);
+}
+
+template <bool A_MN, bool B_MN, bool kPair>
+int launch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
+           const f8::Out& out, int* status, int sms, cudaStream_t stream) {
+  using TL = f8::Tile<kPair>;
+  CUtensorMap mapA, mapB;
+  if (int rc = tc::encode_operand_map8(&mapA, a, f8::kBM)) return rc;
+  if (int rc = tc::encode_operand_map8(&mapB, b, TL::kBRows)) return rc;
+  auto kern = f8::gemm_fp8_kernel<A_MN, B_MN, kPair>;
+  static bool attr_set[64];  // per instantiation and device
+  int dev = 0;
+  CLT_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    CLT_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, f8::kSmemBytes));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const long long total = up(g.M, TL::kM) * up(g.N, f8::kBN) * g.nz, workers = sms / TL::kCtas;
+  CLT_CHECK_ARG(total < (1ll << 31), "fp8_matmul: too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((total < workers ? total : workers) * TL::kCtas));
+  cfg.blockDim = dim3(f8::kThreads);
+  cfg.dynamicSmemBytes = f8::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = TL::kCtas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = kPair ? 1 : 0;
+  CLT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, mapA, mapB, g, sa, sb, out, status));
+  return 0;
+}
+
+int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
+             const f8::Out& out, int* status, int sms, cudaStream_t stream) {
+  const bool pair = use_pair(g, sms);
+#define CLT_FP8_CASE(AM, BM)                                                                                   \
+  if ((a.mn_major != 0) == AM && (b.mn_major != 0) == BM)                                                      \
+    return pair ? launch<AM, BM, true>(g, a, b, sa, sb, out, status, sms, stream)                              \
+                : launch<AM, BM, false>(g, a, b, sa, sb, out, status, sms, stream);
+  CLT_FP8_CASE(false, false)
+  CLT_FP8_CASE(false, true)
+  CLT_FP8_CASE(true, false)
+  CLT_FP8_CASE(true, true)
+#undef CLT_FP8_CASE
+  return 1;
+}
+
+bool geom(GemmGeom& g, int mode, int M, int N, int K, int L) {
+  if (mode < 0 || mode > 3 || M <= 0 || N <= 0 || K <= 0 || L <= 0 || L > 4096) return false;
+  g = GemmGeom{mode, M, N, K, L, mode == kDecDW ? L * (L + 1) / 2 : L};
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int clt_fp8_matmul_parts(int mode, int M, int N, int K, int L, int num_sms) {
+  GemmGeom g;
+  if (!geom(g, mode, M, N, K, L)) return 0;
+  return plan_parts(g, num_sms > 0 ? num_sms : device_sm_count());
+}
+
+int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_trans, const float* sa, int64_t sa_z,
+                   int64_t sa_mn, int64_t sa_k, int a_rows, const void* b, int64_t b_ld, int64_t b_z, int b_trans,
+                   const float* sb, int64_t sb_z, int64_t sb_mn, int64_t sb_k, const float* bias, int64_t bias_z, void* out,
+                   int out_dtype, int64_t out_ld, int64_t out_z, float* ws, int64_t ws_floats, int M, int N, int K, int L,
+                   int* status, clt_stream_t stream) {
+  GemmGeom g;
+  CLT_CHECK_ARG(geom(g, mode, M, N, K, L), "fp8_matmul: bad mode %d or dims M=%d N=%d K=%d L=%d", mode, M, N, K, L);
+  CLT_CHECK_ARG(a && b && sa && sb && out && status, "fp8_matmul: null pointer");
+  CLT_CHECK_ARG(out_dtype >= 0 && out_dtype <= 2, "fp8_matmul: output type %d", out_dtype);
+  CLT_CHECK_ARG(a_rows == 128 || (a_rows == 1 && !a_trans),
+                "fp8_matmul: blocks of %d rows (1 or 128; a transposed operand needs 128)", a_rows);
+  CLT_CHECK_ARG(out_ld >= N, "fp8_matmul: rows of %d values at a distance of %lld", N, (long long)out_ld);
+  const int esize = out_dtype == 0 ? 4 : 2, sms = device_sm_count();
+  CLT_CHECK_ARG((uintptr_t)out % esize == 0, "fp8_matmul: misaligned output");
+  // stacked matrices: [L] each, but the decoder's blocks, which are [pairs]
+  const long long pairs = (long long)L * (L + 1) / 2;
+  const long long na = L, nb = mode == kDecFwd || mode == kDecDFeat ? pairs : L;
+  tc::TcOperand ta{a, a_trans ? 1 : 0, a_trans ? M : K, a_trans ? K : M, a_ld, na, a_z};
+  tc::TcOperand tb{b, b_trans ? 0 : 1, b_trans ? K : N, b_trans ? N : K, b_ld, nb, b_z};
+  const f8::Scales fa{sa, sa_z, sa_mn, sa_k, a_rows == 1 ? 0 : 7}, fb{sb, sb_z, sb_mn, sb_k, 7};
+  f8::Out fo{out, out_dtype, out_ld, out_z, bias, bias_z, 0};
+  fo.aligned = (uintptr_t)out % 16 == 0 && out_ld * esize % 16 == 0 && (g.nz == 1 || out_z * esize % 16 == 0);
+  const long long slab = (long long)M * N;
+  if (ws != nullptr) {
+    CLT_CHECK_ARG((uintptr_t)ws % 16 == 0, "fp8_matmul: the workspace must be 16-byte aligned");
+    GemmGeom gp = g;
+    const int parts = plan_parts(gp, sms);
+    if (parts > 0 && parts * slab <= ws_floats) {
+      gp.nz = parts;
+      const f8::Out po{ws, 0, N, slab, nullptr, 0, N % 4 == 0};
+      if (int rc = dispatch(gp, ta, tb, fa, fb, po, status, sms, (cudaStream_t)stream)) return rc;
+      const dim3 grid((unsigned)up(slab, 256), g.nz);
+      const int kps = (int)up(K, f8::kBK);
+      gp.nz = g.nz;
+      if (out_dtype == 0)
+        fp8_sum_parts_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
+      else if (out_dtype == 1)
+        fp8_sum_parts_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
+      else
+        fp8_sum_parts_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
+      CLT_CHECK_CUDA(cudaGetLastError());
+      return 0;
+    }
+  }
+  return dispatch(g, ta, tb, fa, fb, fo, status, sms, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -74,6 +74,27 @@ int encode_operand_map(CUtensorMap* map, const TcOperand& o, int tile_rows_if_k_
   return 0;
 }
 
+// The same of single bytes: one box of 128 x tile_rows, or boxes of 128 x 128.
+int encode_operand_map8(CUtensorMap* map, const TcOperand& o, int tile_rows_if_k_major) {
+  EncodeTiledFn fn = encode_fn();
+  CLT_CHECK_ARG(fn != nullptr, "cuTensorMapEncodeTiled is not available from this driver");
+  CLT_CHECK_ARG(((uintptr_t)o.ptr & 15) == 0, "8-bit operand must be 16-byte aligned");
+  CLT_CHECK_ARG(o.inner > 0 && o.rows > 0 && o.z_count > 0, "empty 8-bit operand");
+  CLT_CHECK_ARG(o.row_stride % 16 == 0 && o.row_stride >= o.inner && (o.z_count == 1 || (o.z_stride % 16 == 0 && o.z_stride > 0)),
+                "8-bit operand: distances of rows (%lld, %lld values each) and matrices (%lld) must be multiples of 16",
+                o.row_stride, o.inner, o.z_stride);
+  cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.rows, (cuuint64_t)o.z_count};
+  cuuint64_t strides[2] = {(cuuint64_t)o.row_stride, (cuuint64_t)(o.z_count > 1 ? o.z_stride : o.row_stride * o.rows)};
+  cuuint32_t box[3] = {128, (cuuint32_t)(o.mn_major ? 128 : tile_rows_if_k_major), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(o.ptr), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CLT_CHECK_ARG(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d (inner %lld rows %lld z %lld)", (int)r,
+                o.inner, o.rows, o.z_count);
+  return 0;
+}
+
 }  // namespace tc
 }  // namespace clt
 

@@ -476,6 +476,55 @@ int clt_adam_step(float* p, const float* g, float* m, float* v, void* shadow_bf1
 /* fp32 -> bf16 copy of a parameter buffer (the tensor-core operands). */
 int clt_cast_bf16(const float* src, void* dst, int64_t n, clt_stream_t stream);
 
+/* ---- 8-bit operands and checkpoints ---------------------------------------------------------
+ * e4m3 values (finite range +-448, 0x7f = NaN) with an fp32 scale for each block of 1 x 128 or 128 x 128 of a matrix [R, C]:
+ * a value stands for value * scale.  Blocks start at the matrix's origin, the last ones may be cut off.  Strides and `ld` count
+ * elements.  dtype: 0 = fp32, 1 = fp16, 2 = bf16, as in_dtype.  The reference has no counterpart; the products are those of
+ * its encoder and decoders (crosslayer_transcoder/model/clt.py:157-165, 241-248, 334-343) and what autograd derives of them. */
+
+/* x [Z, R, C] (rows ld apart, matrices z_stride; 0 is a broadcast) -> q [Z, R, q_ld], scales [Z, ceil(R / block_rows),
+ * ceil(C / 128)].  scale = the smallest power of two s >= 2^-126 with amax / s <= 448, amax over the block's finite values (1 where
+ * all are 0); value = x / s rounded to e4m3, NaN for what is not finite.  q is 16-byte aligned with q_ld >= C a multiple of 16,
+ * zeros behind a row's end up to the next multiple of 8.  column_sums (blocks of 128 rows only, may be NULL) [Z, ceil(R / 128),
+ * C]: sums of x over each block's rows; clt_sum_chunks adds them up: out[z, c] = sum over the chunks, in their order. */
+int clt_fp8_quantize(const void* x, int in_dtype, int64_t ld, int64_t z_stride, void* q, int64_t q_ld, float* scales,
+                     float* column_sums, int Z, int R, int C, int block_rows, clt_stream_t stream);
+int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_stream_t stream);
+/* out [Z, R, C] (contiguous) = value * scale, rounded once.  s_z, s_r, s_c: distances of the scales between matrices, blocks
+ * of rows and blocks of columns. */
+int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,
+                       int block_rows, void* out, int out_dtype, int Z, int R, int C, clt_stream_t stream);
+
+/* out[z] = A B + bias[z] over slabs z, in fp32 sums, rounded once to out_dtype.  A [M, K] (a_trans: stored [K, M]) with blocks of
+ * a_rows x 128 (a_trans: 128 x 128), B [K, N] (b_trans: stored [N, K]) with blocks of 128 x 128; a_mn / a_k: distances of the
+ * scales between blocks along M and along K, likewise for B along N and K.  Any fp32 scales will do whose products are finite.
+ *   mode 0: L slabs, A and B stacked [L]
+ *   mode 1: slab t of L sums A[s] B[pair(t, s)] over s <= t (crosslayer decoder)
+ *   mode 2: slab s of L sums A[t] B[pair(t, s)] over t >= s (its feature gradient)
+ *   mode 3: slab pair(t, s) of L (L + 1) / 2 is A[s] B[t] (its weight gradient),      pair(t, s) = t (t + 1) / 2 + s
+ * Rows and matrices of a and b start on 16 bytes (a_ld, a_z, b_ld, b_z multiples of 16).  out: rows out_ld apart, slabs out_z.
+ * ws (16-byte aligned, may be NULL): scratch for partial sums of a contraction that is cut into parts; with fewer than
+ * clt_fp8_matmul_parts(...) * M * N floats every output is one chain.  clt_fp8_matmul_parts launches nothing (num_sms 0: the
+ * current device). */
+int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_trans, const float* sa, int64_t sa_z,
+                   int64_t sa_mn, int64_t sa_k, int a_rows, const void* b, int64_t b_ld, int64_t b_z, int b_trans,
+                   const float* sb, int64_t sb_z, int64_t sb_mn, int64_t sb_k, const float* bias, int64_t bias_z, void* out,
+                   int out_dtype, int64_t out_ld, int64_t out_z, float* ws, int64_t ws_floats, int M, int N, int K, int L,
+                   int* status, clt_stream_t stream);
+int clt_fp8_matmul_parts(int mode, int M, int N, int K, int L, int num_sms);
+
+/* JumpReLU (theta [C]) or ReLU (theta NULL) of x [R, C] (rows ld apart; crosslayer_transcoder/model/jumprelu.py:17-48) with a
+ * checkpoint of two bits a value instead of x: y [R, C] = x where x > theta and x > 0, else 0 (NaN stays NaN); bits: ceil(C / 8)
+ * 16-bit words a row.  Backward: dx = g where x >= 0 (ReLU: x > 0), dtheta[c] = -(theta / bandwidth) sum of g where theta -
+ * bandwidth / 2 < x <= theta + bandwidth / 2.  bandwidth: one fp32 value on the device, or NULL for bandwidth_value.  ws:
+ * clt_jump_relu_chunks(R, C) * C floats of scratch for the sums (theta given).  dtype is that of x, y, g and dx. */
+int clt_jump_relu_fwd(const void* x, int64_t ld, const float* theta, const float* bandwidth, float bandwidth_value, void* y,
+                      void* bits, int dtype, int R, int C, clt_stream_t stream);
+int clt_jump_relu_bwd(const void* g, int64_t ld, const void* bits, const float* theta, const float* bandwidth,
+                      float bandwidth_value, void* dx, float* dtheta, float* ws, int64_t ws_floats, int dtype, int R, int C,
+                      clt_stream_t stream);
+int clt_jump_relu_chunks(int R, int C);
+
 #ifdef __cplusplus
 }
 #endif
