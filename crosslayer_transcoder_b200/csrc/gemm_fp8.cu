@@ -69,14 +69,17 @@ __global__ void __launch_bounds__(256) fp8_sum_parts_kernel(const float* __restr
   ((T*)out.p)[z * out.z + m * out.ld + n] = FromFloat<T>::get(acc);
 }
 
-template <bool A_MN, bool B_MN, bool kPair>
-int launch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
-           const f8::Out& out, int* status, int sms, cudaStream_t stream) {
+template <bool A_MN, bool B_MN, bool kPair, int kOut>
+int launch_one(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
+               const f8::Out& out, int* status, int sms, cudaStream_t stream) {
   using TL = f8::Tile<kPair>;
   CUtensorMap mapA, mapB;
   if (int rc = tc::encode_operand_map8(&mapA, a, f8::kBM)) return rc;
   if (int rc = tc::encode_operand_map8(&mapB, b, TL::kBRows)) return rc;
-  auto kern = f8::gemm_fp8_kernel<A_MN, B_MN, kPair>;
+  CUtensorMap mapOut = mapA;  // (not used where rows are not aligned)
+  if (out.tma)
+    if (int rc = tc::encode_output_map(&mapOut, out.p, out.dtype, g.N, g.M, g.nz, out.ld, out.z)) return rc;
+  auto kern = f8::gemm_fp8_kernel<A_MN, B_MN, kPair, kOut>;
   static bool attr_set[64];  // per instantiation and device
   int dev = 0;
   CLT_CHECK_CUDA(cudaGetDevice(&dev));
@@ -96,8 +99,16 @@ int launch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, co
   at.val.clusterDim.x = TL::kCtas, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = kPair ? 1 : 0;
-  CLT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, mapA, mapB, g, sa, sb, out, status));
+  CLT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, mapA, mapB, mapOut, g, sa, sb, out, status));
   return 0;
+}
+
+template <bool A_MN, bool B_MN, bool kPair>
+int launch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
+           const f8::Out& out, int* status, int sms, cudaStream_t stream) {
+  if (out.dtype == 0) return launch_one<A_MN, B_MN, kPair, 0>(g, a, b, sa, sb, out, status, sms, stream);
+  if (out.dtype == 1) return launch_one<A_MN, B_MN, kPair, 1>(g, a, b, sa, sb, out, status, sms, stream);
+  return launch_one<A_MN, B_MN, kPair, 2>(g, a, b, sa, sb, out, status, sms, stream);
 }
 
 int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
@@ -152,7 +163,7 @@ int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_tra
   tc::TcOperand tb{b, b_trans ? 0 : 1, b_trans ? K : N, b_trans ? N : K, b_ld, nb, b_z};
   const f8::Scales fa{sa, sa_z, sa_mn, sa_k, a_rows == 1 ? 0 : 7}, fb{sb, sb_z, sb_mn, sb_k, 7};
   f8::Out fo{out, out_dtype, out_ld, out_z, bias, bias_z, 0};
-  fo.aligned = (uintptr_t)out % 16 == 0 && out_ld * esize % 16 == 0 && (g.nz == 1 || out_z * esize % 16 == 0);
+  fo.tma = (uintptr_t)out % 16 == 0 && out_ld * esize % 16 == 0 && (g.nz == 1 || (out_z > 0 && out_z * esize % 16 == 0));
   const long long slab = (long long)M * N;
   if (ws != nullptr) {
     CLT_CHECK_ARG((uintptr_t)ws % 16 == 0, "fp8_matmul: the workspace must be 16-byte aligned");

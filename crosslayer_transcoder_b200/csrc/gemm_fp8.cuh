@@ -31,12 +31,12 @@ using tc::kEpiThreads;
 using tc::kEpiWarps;
 using tc::kFirstEpiWarp;
 using tc::kMaxStages;
-using tc::kRegsEpi;
-using tc::kRegsLean;
 using tc::kThreads;
 using tc::kTmemCols;
 constexpr int kBK = 128;         // contraction of a stage = of a scale block
 constexpr int kBox = 128 * 128;  // bytes of one box
+constexpr int kRegsLean = 56, kRegsEpi = 224;  // 128 * 56 + 256 * 224 = 384 * 168, what the block is launched with
+constexpr int kBatch = 8;        // blocks whose scales are handed to the epilogue together
 
 template <bool kPair>
 struct Tile {
@@ -46,14 +46,24 @@ struct Tile {
   static constexpr int kABytes = kBM * kBK;
   static constexpr int kBBytes = kBRows * kBK;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStages = kPair ? 4 : 3;  // (six and four, without room for the output, were no faster)
 };
-constexpr int kOperandBytes = Tile<true>::kStages * Tile<true>::kStageBytes;
-static_assert(kOperandBytes == Tile<false>::kStages * Tile<false>::kStageBytes, "both forms fill the same memory");
-constexpr int kBiasBytes = kEpiWarps * 128 * 4;  // each warp's own columns
+constexpr int kOperandBytes = 144 * 1024;
+static_assert(Tile<true>::kStages * Tile<true>::kStageBytes <= kOperandBytes &&
+                  Tile<false>::kStages * Tile<false>::kStageBytes <= kOperandBytes,
+              "operand stages");
+constexpr int kOutBytes = 8 * 1024;  // a warp's output on its way to memory: two boxes of 32 rows x 128 B
+// Scales of two batches, of the tile's 128 rows and of its two halves of the columns, and the bias of two tiles.
+struct ScaleRing {
+  float a[2][kBatch][128];
+  float b[2][kBatch][2];
+  float bias[2][kBN];
+  uint64_t full[2], empty[2];
+};
 constexpr int kSmemBytes =
-    kOperandBytes + 1024 /*alignment slack*/ + 256 /*barriers*/ + kBiasBytes + kEpiWarps * epi::kStageBytes;
-static_assert(sizeof(tc::Barriers) <= 256, "barriers");
+    kOperandBytes + kEpiWarps * kOutBytes + 1024 /*alignment slack*/ + 256 /*barriers*/ + (int)sizeof(ScaleRing);
+static_assert(sizeof(tc::Barriers) <= 256 && sizeof(ScaleRing) % 16 == 0 && kSmemBytes <= 232448, "shared memory");
+constexpr int kScaleWarps = 2;  // warps 2 and 3
 
 // Scales of one operand: element strides between matrices, between blocks along M (or N) and along K.
 struct Scales {
@@ -68,8 +78,62 @@ struct Out {
   long long ld, z;
   const float* bias;  // [nz, N] or NULL
   long long bias_z;
-  int aligned;  // rows of every slab start on 16 bytes
+  int tma;  // rows of every slab start on 16 bytes: copied out by TMA
 };
+
+// Waits and arrivals at CTA scope, also where the barrier is the other CTA's: what they order are reads of tensor memory, which
+// tcgen05's own fences cover, and no other data passes from CTA to CTA.  At cluster scope (gemm_tc.cuh, once a tile) each arrival
+// is a memory fence behind every load in flight and each wait drops the L1 that holds the scales: 8192^3 887 instead of
+// 1543 TFLOP/s.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (try_wait(bar, parity)) return true;
+    if (*abort_flag != 0) return false;
+    if (clock64() - t0 > tc::kWaitCycles) {
+      report_status(status, code);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+// Whether the n-th block's products are in tensor memory; uniform over the warp.  All lanes look: one that tells the others costs
+// more, each block (8192^3: 463 -> 587 us without the sums).
+__device__ __forceinline__ bool block_ready(tc::Barriers* bars, uint32_t n, volatile int* abort_flag, int* status) {
+  const bool ok = wait(tc::smem_u32(&bars->tmem_full[n & 1]), (n >> 1) & 1, abort_flag, status, kTimeoutTmemFull);
+  if (!__all_sync(0xffffffffu, ok)) return false;
+  tc::tc_fence_after();
+  return true;
+}
+// One lane of a converged warp.  A role's warp runs its loop as a whole and only what must not happen 32 times is under this: the
+// loop's values then stay in uniform registers, where the MMAs and copies want them (a loop in one lane alone: 2208 instead of
+// 2450 TFLOP/s at 12 x 4000 x 24576 x 768, without the sums).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 template <bool kPair>
 __device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
@@ -96,6 +160,8 @@ __host__ __device__ constexpr uint32_t instr_desc(bool a_mn, bool b_mn, int m) {
          ((uint32_t)(m >> 4) << 24);
 }
 
+// Asynchronous read of 16 accumulator columns of this warp's 32 lanes; valid after tmem_ld_wait(r), through which the values pass so
+// that nothing that uses them is moved ahead of it.
 __device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -105,8 +171,6 @@ __device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16
       : "r"(taddr)
       : "memory");
 }
-
-// Waits for this warp's reads of tensor memory.  The registers are operands so that nothing that uses them is moved ahead.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -114,20 +178,9 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
                :
                : "memory");
 }
-
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-  return d;
-}
-__device__ __forceinline__ void unpack2(uint64_t d, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(d));
-}
-// acc += d * s, two at a time
-__device__ __forceinline__ void fma16(uint64_t* acc, const uint32_t (&d)[16], uint64_t s2) {
+__device__ __forceinline__ void fma16(float* acc, const uint32_t (&d)[16], float s) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i]) : "l"(pack2(d[2 * i], d[2 * i + 1])), "l"(s2));
+  for (int i = 0; i < 16; ++i) acc[i] = fmaf(__uint_as_float(d[i]), s, acc[i]);
 }
 
 // ---- stores -------------------------------------------------------------------------------------
@@ -141,60 +194,93 @@ __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A warp's 32 x 32 sub-tile of 16-bit values, as epi::store_rows32; rows that are not 16-byte aligned or that end inside the
-// sub-tile go out one row to an instruction.
-template <class T>
-__device__ __forceinline__ void store16(unsigned char* stage, T* base, long long ld, int rows_valid, int cols_valid,
-                                        bool aligned, const float (&v)[32]) {
+// 16 bytes of finished sums in the output's type: 4 fp32, 8 16-bit values
+template <int kOut>
+__device__ __forceinline__ uint4 pack_out(const float* v) {
+  if constexpr (kOut == 0)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else if constexpr (kOut == 1)
+    return make_uint4(pack16<__half>(v[0], v[1]), pack16<__half>(v[2], v[3]), pack16<__half>(v[4], v[5]), pack16<__half>(v[6], v[7]));
+  else
+    return make_uint4(pack16<__nv_bfloat16>(v[0], v[1]), pack16<__nv_bfloat16>(v[2], v[3]), pack16<__nv_bfloat16>(v[4], v[5]),
+                      pack16<__nv_bfloat16>(v[6], v[7]));
+}
+
+template <int kKeep>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kKeep) : "memory");
+}
+
+// A warp's 32 rows x 128 columns of finished sums, to the output in the type kOut (as Out::dtype; one instantiation each: with all
+// three in one kernel the sums do not stay in registers).  Boxes of 32 rows x 128 B go through two buffers of shared memory
+// (128-byte swizzle: conflict-free 16-byte stores, a row per lane) and out by TMA, which clips what lies behind the matrix's
+// end; the warp does not wait for its last two.  Rows that do not start on 16 bytes are written from the buffers by the warp.
+// (16-byte stores from registers through a small buffer, as in epi::store_rows32, took 2.4 us a tile, in which the tensor cores wait:
+// 12 x 4000 x 768 x 24576 1643 instead of 1318 us.)
+template <int kOut>
+__device__ __forceinline__ void store_warp(float (&acc)[128], const float* bias, uint8_t* buf, const CUtensorMap* map, const Out& o,
+                                           int z, int row0, int col0, int M, int N) {
+  constexpr int kSize = kOut == 0 ? 4 : 2, kCols = 128 / kSize, kPer = 16 / kSize;
   const int lane = threadIdx.x & 31;
-  uint4* mine = reinterpret_cast<uint4*>(stage + lane * epi::kStageRow);
+  if (o.bias != nullptr) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    mine[i] = make_uint4(pack16<T>(v[8 * i], v[8 * i + 1]), pack16<T>(v[8 * i + 2], v[8 * i + 3]),
-                         pack16<T>(v[8 * i + 4], v[8 * i + 5]), pack16<T>(v[8 * i + 6], v[8 * i + 7]));
-  __syncwarp();
-  if (aligned && cols_valid >= 32) {
-    const int piece = lane & 3;
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int r = it * 8 + (lane >> 2);
-      const uint4 t = *reinterpret_cast<const uint4*>(stage + r * epi::kStageRow + piece * 16);
-      if (r < rows_valid) *reinterpret_cast<uint4*>(base + r * ld + piece * 8) = t;
+    for (int i = 0; i < 32; ++i) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
+      acc[4 * i] += b.x, acc[4 * i + 1] += b.y, acc[4 * i + 2] += b.z, acc[4 * i + 3] += b.w;
     }
-  } else if (lane < cols_valid) {
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r)
-      if (r < rows_valid) base[r * ld + lane] = *reinterpret_cast<const T*>(stage + r * epi::kStageRow + lane * 2);
   }
-  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 128 / kCols; ++c) {
+    uint8_t* box = buf + (c & 1) * 4096;
+    if (lane == 0) bulk_wait_read<1>();  // the copy before last, from this buffer, has been read
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = pack_out<kOut>(acc + c * kCols + i * kPer);
+    const int n = col0 + c * kCols;
+    if (o.tma) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        if (n < N)
+          asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                       "r"(tc::smem_u32(box)), "r"(n), "r"(row0), "r"(z)
+                       : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else {
+      __syncwarp();
+      const int rows = min(32, M - row0), cols = min(kCols, N - n);
+      uint8_t* p = (uint8_t*)o.p + (z * o.z + (long long)row0 * o.ld + n) * kSize;
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+#pragma unroll
+        for (int k = lane; k < kCols; k += 32) {
+          if (k < cols) {
+            const uint8_t* v = box + r * 128 + (((k / kPer) ^ (r & 7)) << 4) + k % kPer * kSize;
+            if constexpr (kOut == 0)
+              *reinterpret_cast<uint32_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint32_t*>(v);
+            else
+              *reinterpret_cast<uint16_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint16_t*>(v);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
 }
 
-__device__ __forceinline__ void store_chunk(unsigned char* stage, const Out& o, int z, int row0, int n, int M, int N,
-                                            const float (&v)[32]) {
-  const long long at = z * o.z + (long long)row0 * o.ld + n;
-  const int rows = M - row0, cols = N - n;
-  if (o.dtype == 0) {
-    float* p = (float*)o.p + at;
-    if (o.aligned && cols >= 32)
-      epi::store_rows32<float>(stage, p, (size_t)o.ld, rows, v);
-    else
-      epi::store_rows32_scalar(stage, p, (size_t)o.ld, rows, cols, v);
-  } else if (o.dtype == 1) {
-    store16<__half>(stage, (__half*)o.p + at, o.ld, rows, cols, o.aligned != 0, v);
-  } else {
-    store16<__nv_bfloat16>(stage, (__nv_bfloat16*)o.p + at, o.ld, rows, cols, o.aligned != 0, v);
-  }
-}
-
-template <bool A_MN, bool B_MN, bool kPair>
+template <bool A_MN, bool B_MN, bool kPair, int kOut>
 __global__ void __launch_bounds__(kThreads, 1)
-gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB, GemmGeom g,
-                Scales sa, Scales sb, Out out, int* status) {
+gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
+                const __grid_constant__ CUtensorMap mapOut, GemmGeom g, Scales sa, Scales sb, Out out, int* status) {
   extern __shared__ uint8_t smem_raw[];
   using TL = Tile<kPair>;
   constexpr int kStages = TL::kStages, kStageBytes = TL::kStageBytes, kABytes = TL::kABytes;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  tc::Barriers* bars = reinterpret_cast<tc::Barriers*>(smem + kOperandBytes);
+  uint8_t* out_smem = smem + kOperandBytes;
+  tc::Barriers* bars = reinterpret_cast<tc::Barriers*>(out_smem + kEpiWarps * kOutBytes);
+  ScaleRing* ring = reinterpret_cast<ScaleRing*>(out_smem + kEpiWarps * kOutBytes + 256);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -217,6 +303,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
       tc::mbar_init(tc::smem_u32(&bars->tmem_full[i]), 1);
       tc::mbar_init(tc::smem_u32(&bars->tmem_empty[i]), TL::kCtas * kEpiWarps);
     }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(tc::smem_u32(&ring->full[i]), kScaleWarps);
+      tc::mbar_init(tc::smem_u32(&ring->empty[i]), kEpiWarps);
+    }
     bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -237,34 +327,39 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLean));
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
-      if (lane == 0) {
-        int stage = 0;
-        uint32_t phase = 0;
-        bool alive = true;
-        for (int i = 0; alive; ++i) {
-          const long long tile_l = tc::tile_of_round(i, worker, workers);
-          if (tile_l >= total_tiles) break;
-          const int tile = (int)tile_l;
-          int z, kb_lo, kb_hi, zo;
-          work_item(g, tile / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
-          int m0, n0;
-          tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
-          m0 += rank * kBM;
-          n0 += rank * TL::kBRows;
-          int left = kb_hi - kb_lo, kb0 = kb_lo % kb_per_seg;
-          for (int j = kb_lo / kb_per_seg; left > 0 && alive; ++j) {
-            int za, zb;
-            seg_index(g, z, j, za, zb);
-            const int kb1 = min(kb_per_seg, kb0 + left);
-            left -= kb1 - kb0;
-            for (int kb = kb0; kb < kb1; ++kb) {
-              if (!tc::mbar_wait(tc::smem_u32(&bars->empty[stage]), phase ^ 1, abort_flag, status, kTimeoutEmpty)) {
-                alive = false;
-                break;
-              }
-              const uint32_t own = tc::smem_u32(&bars->full[stage]), full = kPair ? tc::cluster_addr(own, 0) : own;
-              if (rank == 0) tc::mbar_expect_tx(own, TL::kCtas * kStageBytes);
-              const uint32_t pa = tc::smem_u32(smem + stage * kStageBytes);
+      const bool one = elect_one();
+      const uint32_t full0 = tc::smem_u32(&bars->full[0]), empty0 = tc::smem_u32(&bars->empty[0]);
+      const uint32_t lead0 = kPair ? tc::cluster_addr(full0, 0) : full0;  // the leader's barriers count the bytes of both
+      const uint32_t stage0 = tc::smem_u32(smem);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool alive = true;
+      for (int i = 0; alive; ++i) {
+        const long long tile_l = tc::tile_of_round(i, worker, workers);
+        if (tile_l >= total_tiles) break;
+        const int tile = (int)tile_l;
+        int z, kb_lo, kb_hi, zo;
+        work_item(g, tile / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
+        int m0, n0;
+        tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
+        m0 += rank * kBM;
+        n0 += rank * TL::kBRows;
+        int left = kb_hi - kb_lo, kb0 = kb_lo % kb_per_seg;
+        for (int j = kb_lo / kb_per_seg; left > 0 && alive; ++j) {
+          int za, zb;
+          seg_index(g, z, j, za, zb);
+          const int kb1 = min(kb_per_seg, kb0 + left);
+          left -= kb1 - kb0;
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (!wait(empty0 + 8 * stage, phase ^ 1, abort_flag, status, kTimeoutEmpty)) {
+              alive = false;
+              break;
+            }
+            __syncwarp();
+            if (one) {
+              const uint32_t full = lead0 + 8 * stage;
+              if (rank == 0) tc::mbar_expect_tx(full0 + 8 * stage, TL::kCtas * kStageBytes);
+              const uint32_t pa = stage0 + stage * kStageBytes;
               const uint32_t pb = pa + kABytes;
               const int k0 = kb * kBK;
               if (A_MN)
@@ -278,30 +373,40 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
               } else {
                 tc::tma_load_3d<kPair>(pb, &mapB, full, k0, n0, zb);
               }
-              if (++stage == kStages) stage = 0, phase ^= 1;
             }
-            kb0 = 0;
-          }
-        }
-        if constexpr (kPair) {
-          // the leader's MMAs read this CTA's stages and its commits arrive here: stay until the last has
-          for (int i = 0; i < kStages && alive; ++i) {
-            alive = tc::mbar_wait(tc::smem_u32(&bars->empty[stage]), phase ^ 1, abort_flag, status, kTimeoutEmpty);
+            __syncwarp();
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
+          kb0 = 0;
         }
-        if (!alive) {
-          // let copies that are still in flight land before the CTA's shared memory goes away
-          const long long t0 = clock64();
-          while (clock64() - t0 < 2000000ll) {
-          }
+        alive = __all_sync(0xffffffffu, alive);
+      }
+      if constexpr (kPair) {
+        // the leader's MMAs read this CTA's stages and its commits arrive here: stay until the last has
+        for (int i = 0; i < kStages && alive; ++i) {
+          alive = wait(empty0 + 8 * stage, phase ^ 1, abort_flag, status, kTimeoutEmpty);
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+      }
+      if (!alive) {
+        // let copies that are still in flight land before the CTA's shared memory goes away
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000ll) {
         }
       }
       __syncwarp();
     } else if (warp == 1) {
       // ------------------------------ MMA issuer --------------------------------
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         constexpr uint32_t idesc = instr_desc(A_MN, B_MN, TL::kM);
+        const bool one = elect_one();
+        const uint32_t full0 = tc::smem_u32(&bars->full[0]), empty0 = tc::smem_u32(&bars->empty[0]);
+        const uint32_t acc_full0 = tc::smem_u32(&bars->tmem_full[0]), acc_empty0 = tc::smem_u32(&bars->tmem_empty[0]);
+        // descriptors of the first stage; a stage further, or a K step, moves their addresses (in 16-byte units)
+        const uint64_t da0 = A_MN ? tc::smem_desc(tc::smem_u32(smem), kBox, 1024) : tc::smem_desc(tc::smem_u32(smem), 16, 1024);
+        const uint64_t db0 = B_MN ? tc::smem_desc(tc::smem_u32(smem) + kABytes, kBox, 1024)
+                                  : tc::smem_desc(tc::smem_u32(smem) + kABytes, 16, 1024);
+        constexpr int kStepA = (A_MN ? 4096 : 32) / 16, kStepB = (B_MN ? 4096 : 32) / 16;
         int stage = 0;
         uint32_t phase = 0;
         uint32_t n = 0;  // blocks so far: accumulator n & 1, used for the (n >> 1)-th time
@@ -312,43 +417,97 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           int z, kb_lo, kb_hi, zo;
           work_item(g, (int)tile_l / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
           for (int kb = kb_lo; kb < kb_hi; ++kb, ++n) {
-            const int buf = n & 1;
-            if (!tc::mbar_wait(tc::smem_u32(&bars->tmem_empty[buf]), ((n >> 1) & 1) ^ 1, abort_flag, status,
-                               kTimeoutTmemEmpty) ||
-                !tc::mbar_wait(tc::smem_u32(&bars->full[stage]), phase, abort_flag, status, kTimeoutFull)) {
+            const uint32_t buf = n & 1;
+            if (!wait(acc_empty0 + 8 * buf, ((n >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty) ||
+                !wait(full0 + 8 * stage, phase, abort_flag, status, kTimeoutFull)) {
               alive = false;
               break;
             }
+            __syncwarp();
             tc::tc_fence_after();
-            const uint32_t pa = tc::smem_u32(smem + stage * kStageBytes);
-            const uint32_t pb = pa + kABytes;
-            const uint32_t tmem_d = tmem_base + buf * kBN;
+            if (one) {
+              const uint32_t tmem_d = tmem_base + buf * kBN;
+              const uint64_t da = da0 + (uint32_t)(stage * (kStageBytes / 16)), db = db0 + (uint32_t)(stage * (kStageBytes / 16));
 #pragma unroll
-            for (int k = 0; k < kBK / 32; ++k) {
-              const uint64_t da =
-                  A_MN ? tc::smem_desc(pa + k * 4096, kBox, 1024) : tc::smem_desc(pa + k * 32, 16, 1024);
-              const uint64_t db =
-                  B_MN ? tc::smem_desc(pb + k * 4096, kBox, 1024) : tc::smem_desc(pb + k * 32, 16, 1024);
-              umma_e4m3<kPair>(tmem_d, da, db, idesc, k > 0 ? 1u : 0u);
+              for (int k = 0; k < kBK / 32; ++k)
+                umma_e4m3<kPair>(tmem_d, da + k * kStepA, db + k * kStepB, idesc, k > 0 ? 1u : 0u);
+              tc::umma_commit<kPair>(empty0 + 8 * stage);
+              tc::umma_commit<kPair>(acc_full0 + 8 * buf);
             }
-            tc::umma_commit<kPair>(tc::smem_u32(&bars->empty[stage]));
-            tc::umma_commit<kPair>(tc::smem_u32(&bars->tmem_full[buf]));
+            __syncwarp();
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
+          alive = __all_sync(0xffffffffu, alive);
         }
       }
       __syncwarp();
+    } else {
+      // ------------------------------ scales ------------------------------------
+      const int t = threadIdx.x - 64;  // rows t and t + 64 of the CTA's 128
+      uint32_t batch = 0;
+      bool alive = true;
+      for (int it = 0; alive; ++it) {
+        const long long tile_l = tc::tile_of_round(it, worker, workers);
+        if (tile_l >= total_tiles) break;
+        const int tile = (int)tile_l;
+        int z, kb_lo, kb_hi, zo, m0, n0;
+        work_item(g, tile / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
+        tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
+        m0 += rank * kBM;
+        // rows and columns behind the end take the last one's: their sums are not stored
+        const float* a0 = sa.p + (long long)(min(m0 + t, g.M - 1) >> sa.shift) * sa.mn;
+        const float* a1 = sa.p + (long long)(min(m0 + t + 64, g.M - 1) >> sa.shift) * sa.mn;
+        const float* b0 = sb.p + (long long)(min(n0 + 128 * (t & 1), g.N - 1) >> 7) * sb.mn;
+        int j = kb_lo / kb_per_seg, kb = kb_lo % kb_per_seg;
+        int za, zb;
+        seg_index(g, z, j, za, zb);
+        for (int left = kb_hi - kb_lo; left > 0; left -= kBatch, ++batch) {
+          const int slot = batch & 1;
+          const bool ok =
+              wait(tc::smem_u32(&ring->empty[slot]), ((batch >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty);
+          alive = __all_sync(0xffffffffu, ok);
+          if (!alive) break;
+          const int n = min(left, kBatch);
+          if (out.bias != nullptr && left == kb_hi - kb_lo) {
+            // with the tile's first batch; the tile before last has given its last batch back, which it does after its output
+#pragma unroll
+            for (int i = 0; i < kBN; i += 64)
+              ring->bias[it & 1][i + t] = n0 + i + t < g.N ? __ldg(out.bias + zo * out.bias_z + n0 + i + t) : 0.f;
+          }
+          float va[kBatch], vb[kBatch], vc[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (i < n) {
+              const long long oa = za * sa.z + kb * sa.k;
+              va[i] = __ldg(a0 + oa), vb[i] = __ldg(a1 + oa);
+              vc[i] = t < 2 ? __ldg(b0 + zb * sb.z + kb * sb.k) : 0.f;
+              if (++kb == kb_per_seg) {
+                kb = 0, ++j;
+                if (i + 1 < left) seg_index(g, z, j, za, zb);
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (i < n) {
+              ring->a[slot][i][t] = va[i], ring->a[slot][i][t + 64] = vb[i];
+              if (t < 2) ring->b[slot][i][t] = vc[i];
+            }
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->full[slot]));
+        }
+      }
     }
   } else {
     // ------------------------------ epilogue ----------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int ew = warp - kFirstEpiWarp;
-    float* bias = reinterpret_cast<float*>(smem + kOperandBytes + 256) + ew * 128;
-    unsigned char* stage = smem + kOperandBytes + 256 + kBiasBytes + ew * epi::kStageBytes;
+    uint8_t* buf8 = out_smem + ew * kOutBytes;
     const int quarter = warp & 3;  // tensor-memory lanes 32*quarter .. +31
     const int half = ew >> 2;      // which 128 columns of the tile
     const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
-    uint32_t n = 0;
+    uint32_t n = 0, batch = 0;
     bool alive = true;
     for (int it = 0; alive; ++it) {
       const long long tile_l = tc::tile_of_round(it, worker, workers);
@@ -360,99 +519,63 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
       tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
       const int row0 = m0 + rank * kBM + quarter * 32, col0 = n0 + half * 128;
       const bool work = row0 < g.M && col0 < g.N;  // uniform over the warp: something of it is stored
-      const long long sa_row = (long long)(min(row0 + lane, g.M - 1) >> sa.shift) * sa.mn;
-      const long long sb_col = (long long)(min(col0, g.N - 1) >> 7) * sb.mn;
-      if (work && out.bias != nullptr) {
-        __syncwarp();
+      float acc[128];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c = col0 + 32 * i + lane;
-          bias[32 * i + lane] = c < g.N ? __ldg(out.bias + zo * out.bias_z + c) : 0.f;
-        }
-        __syncwarp();
-      }
-      uint64_t acc[64];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0;
-      int j = kb_lo / kb_per_seg, kb = kb_lo % kb_per_seg;
-      const float *pa, *pb;
-      float s_next = 0.f;
-      const auto segment = [&]() {
-        int za, zb;
-        seg_index(g, z, j, za, zb);
-        pa = sa.p + za * sa.z + sa_row + kb * sa.k;
-        pb = sb.p + zb * sb.z + sb_col + kb * sb.k;
-      };
-      segment();
-      if (work) s_next = __ldg(pa) * __ldg(pb);
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      uint32_t r0[16], r1[16];
+      // One read of tensor memory is in flight at any time, across the blocks: the next block's first is issued before this
+      // block's last columns are added.
+      alive = block_ready(bars, n, abort_flag, status);
+      if (alive && work) tmem_ld16_issue(tbase + (n & 1) * kBN, r0);
 #pragma unroll 1
-      for (int left = kb_hi - kb_lo; left > 0; --left, ++n) {
-        const float s = s_next;
-        // the next block's scale is on its way while this block is multiplied
-        if (left > 1) {
-          if (++kb == kb_per_seg) {
-            kb = 0, ++j;
-            segment();
-          } else {
-            pa += sa.k, pb += sb.k;
-          }
-          if (work) s_next = __ldg(pa) * __ldg(pb);
-        }
-        const int buf = n & 1;
-        const bool ok =
-            tc::mbar_wait(tc::smem_u32(&bars->tmem_full[buf]), (n >> 1) & 1, abort_flag, status, kTimeoutTmemFull);
-        if (!__all_sync(0xffffffffu, ok)) {
-          alive = false;
-          break;
-        }
-        tc::tc_fence_after();
-        const uint64_t s2 = pack2(__float_as_uint(s), __float_as_uint(s));
-        const uint32_t taddr = tbase + buf * kBN;
-        uint32_t r0[16], r1[16];
-        if (work) {
-          tmem_ld16_issue(taddr, r0);
+      for (int left = kb_hi - kb_lo; left > 0 && alive; left -= kBatch, ++batch) {
+        const int slot = batch & 1;
+        alive = wait(tc::smem_u32(&ring->full[slot]), (batch >> 1) & 1, abort_flag, status, kTimeoutTmemFull);
+        alive = __all_sync(0xffffffffu, alive);
+        const float* ra = &ring->a[slot][0][quarter * 32 + lane];
+        const float* rb = &ring->b[slot][0][half];
+        const int in_batch = min(left, kBatch);
+#pragma unroll 1
+        for (int i = 0; alive && i < in_batch; ++i, ++n) {
+          const float s = ra[i * 128] * rb[i * 2];
+          const int buf = n & 1;
+          const uint32_t taddr = tbase + buf * kBN;
+          if (work) {
 #pragma unroll
-          for (int c = 0; c < 8; c += 2) {
-            tmem_ld_wait(r0);
-            tmem_ld16_issue(taddr + 16 * (c + 1), r1);
-            fma16(acc + 8 * c, r0, s2);
-            tmem_ld_wait(r1);
-            if (c + 2 < 8) {
-              tmem_ld16_issue(taddr + 16 * (c + 2), r0);
-              fma16(acc + 8 * (c + 1), r1, s2);
+            for (int c = 0; c < 8; c += 2) {
+              tmem_ld_wait(r0);
+              tmem_ld16_issue(taddr + 16 * (c + 1), r1);
+              fma16(acc + 16 * c, r0, s);
+              tmem_ld_wait(r1);
+              if (c < 6) {
+                tmem_ld16_issue(taddr + 16 * (c + 2), r0);
+                fma16(acc + 16 * (c + 1), r1, s);
+              }
             }
           }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kPair)
+              arrive_remote(tc::cluster_addr(tc::smem_u32(&bars->tmem_empty[buf]), 0));
+            else
+              tc::mbar_arrive(tc::smem_u32(&bars->tmem_empty[buf]));
+          }
+          if (i + 1 < left) {
+            alive = block_ready(bars, n + 1, abort_flag, status);
+            if (alive && work) tmem_ld16_issue(tbase + ((n + 1) & 1) * kBN, r0);
+          }
+          if (work) fma16(acc + 112, r1, s);
         }
-        tc::tc_fence_before();
+        if (left <= kBatch && alive && work)  // before the slot is given back: the bias that it brought is read here
+          store_warp<kOut>(acc, ring->bias[it & 1] + half * 128, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (kPair)
-            tc::mbar_arrive_cluster(tc::cluster_addr(tc::smem_u32(&bars->tmem_empty[buf]), 0));
-          else
-            tc::mbar_arrive(tc::smem_u32(&bars->tmem_empty[buf]));
-        }
-        if (work) fma16(acc + 56, r1, s2);
-      }
-      if (!alive || !work) continue;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (col0 + 32 * c < g.N) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) unpack2(acc[16 * c + i], v[2 * i], v[2 * i + 1]);
-          if (out.bias != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 b = *reinterpret_cast<const float4*>(bias + 32 * c + 4 * i);
-              v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
-            }
-          }
-          store_chunk(stage, out, zo, row0, col0 + 32 * c, g.M, g.N, v);
-        }
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->empty[slot]));
       }
     }
   }
 
+  if (warp >= kFirstEpiWarp && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   tc::tc_fence_before();
   if constexpr (kPair)
     tc::cluster_sync();

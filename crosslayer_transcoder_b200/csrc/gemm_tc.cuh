@@ -579,6 +579,8 @@ inline bool use_pair(const GemmGeom& g, int num_sms) {
 
 int encode_operand_map(CUtensorMap* map, const TcOperand& o, int tile_rows_if_k_major);
 int encode_operand_map8(CUtensorMap* map, const TcOperand& o, int tile_rows_if_k_major);  // strides in bytes
+int encode_output_map(CUtensorMap* map, void* ptr, int dtype, long long cols, long long rows, long long z, long long ld,
+                      long long z_stride);
 
 template <class Epi, bool A_MN, bool B_MN, bool kPair>
 int launch_gemm_tc_tile(const GemmGeom& g, const TcOperand& a, const TcOperand& b, const typename Epi::Params& ep,

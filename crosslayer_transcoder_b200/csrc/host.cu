@@ -95,6 +95,24 @@ int encode_operand_map8(CUtensorMap* map, const TcOperand& o, int tile_rows_if_k
   return 0;
 }
 
+// Output [z, rows, cols] of type dtype (0 fp32, 1 fp16, 2 bf16), strides in elements; boxes of 32 rows x 128 bytes.
+int encode_output_map(CUtensorMap* map, void* ptr, int dtype, long long cols, long long rows, long long z, long long ld,
+                      long long z_stride) {
+  EncodeTiledFn fn = encode_fn();
+  CLT_CHECK_ARG(fn != nullptr, "cuTensorMapEncodeTiled is not available from this driver");
+  const int e = dtype == 0 ? 4 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)z};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * e, (cuuint64_t)(z > 1 ? z_stride : ld * rows) * e};
+  cuuint32_t box[3] = {(cuuint32_t)(128 / e), 32, 1}, estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype == 0   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                       : dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  3, ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CLT_CHECK_ARG(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code %d (output %lld x %lld x %lld)", (int)r, z, rows, cols);
+  return 0;
+}
+
 }  // namespace tc
 }  // namespace clt
 
