@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(256) fp8_sum_parts_kernel(const float* __restr
   ((T*)out.p)[z * out.z + m * out.ld + n] = FromFloat<T>::get(acc);
 }
 
-template <bool A_MN, bool B_MN, bool kPair, int kOut>
+template <bool A_MN, bool B_MN, bool kPair, int kOut, bool kByRow>
 int launch_one(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
                const f8::Out& out, int* status, int sms, cudaStream_t stream) {
   using TL = f8::Tile<kPair>;
@@ -79,7 +79,7 @@ int launch_one(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b
   CUtensorMap mapOut = mapA;  // (not used where rows are not aligned)
   if (out.tma)
     if (int rc = tc::encode_output_map(&mapOut, out.p, out.dtype, g.N, g.M, g.nz, out.ld, out.z)) return rc;
-  auto kern = f8::gemm_fp8_kernel<A_MN, B_MN, kPair, kOut>;
+  auto kern = f8::gemm_fp8_kernel<A_MN, B_MN, kPair, kOut, kByRow>;
   static bool attr_set[64];  // per instantiation and device
   int dev = 0;
   CLT_CHECK_CUDA(cudaGetDevice(&dev));
@@ -103,27 +103,29 @@ int launch_one(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b
   return 0;
 }
 
-template <bool A_MN, bool B_MN, bool kPair>
+template <bool A_MN, bool B_MN, bool kPair, bool kByRow>
 int launch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
            const f8::Out& out, int* status, int sms, cudaStream_t stream) {
-  if (out.dtype == 0) return launch_one<A_MN, B_MN, kPair, 0>(g, a, b, sa, sb, out, status, sms, stream);
-  if (out.dtype == 1) return launch_one<A_MN, B_MN, kPair, 1>(g, a, b, sa, sb, out, status, sms, stream);
-  return launch_one<A_MN, B_MN, kPair, 2>(g, a, b, sa, sb, out, status, sms, stream);
+  if (out.dtype == 0) return launch_one<A_MN, B_MN, kPair, 0, kByRow>(g, a, b, sa, sb, out, status, sms, stream);
+  if (out.dtype == 1) return launch_one<A_MN, B_MN, kPair, 1, kByRow>(g, a, b, sa, sb, out, status, sms, stream);
+  return launch_one<A_MN, B_MN, kPair, 2, kByRow>(g, a, b, sa, sb, out, status, sms, stream);
 }
 
 int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, const f8::Scales& sa, const f8::Scales& sb,
              const f8::Out& out, int* status, int sms, cudaStream_t stream) {
   const bool pair = use_pair(g, sms);
-#define CLT_FP8_CASE(AM, BM)                                                                                   \
-  if ((a.mn_major != 0) == AM && (b.mn_major != 0) == BM)                                                      \
-    return pair ? launch<AM, BM, true>(g, a, b, sa, sb, out, status, sms, stream)                              \
-                : launch<AM, BM, false>(g, a, b, sa, sb, out, status, sms, stream);
-  CLT_FP8_CASE(false, false)
-  CLT_FP8_CASE(false, true)
-  CLT_FP8_CASE(true, false)
-  CLT_FP8_CASE(true, true)
+#define CLT_FP8_CASE(AM, BM, ROW)                                                                              \
+  if ((a.mn_major != 0) == AM && (b.mn_major != 0) == BM && (sa.shift == 0) == ROW)                            \
+    return pair ? launch<AM, BM, true, ROW>(g, a, b, sa, sb, out, status, sms, stream)                         \
+                : launch<AM, BM, false, ROW>(g, a, b, sa, sb, out, status, sms, stream);
+  CLT_FP8_CASE(false, false, false)
+  CLT_FP8_CASE(false, true, false)
+  CLT_FP8_CASE(true, false, false)
+  CLT_FP8_CASE(true, true, false)
+  CLT_FP8_CASE(false, false, true)
+  CLT_FP8_CASE(false, true, true)
 #undef CLT_FP8_CASE
-  return 1;
+  CLT_CHECK_ARG(false, "fp8_matmul: operand layout");
 }
 
 bool geom(GemmGeom& g, int mode, int M, int N, int K, int L) {

@@ -11,7 +11,11 @@
 //   * A stage holds 128 of the contraction axis, one byte each: as many bytes as 64 bf16 values, twice the products.
 //   * The two accumulators of tensor memory alternate from block to block instead of from tile to tile: while the MMAs fill
 //     one, the eight epilogue warps read the other and add it to their 128 sums a thread (32 rows x 128 columns a warp).
-//     That is 16384 packed FMAs a block and SM, 256 cycles of the fp32 pipes beside 512 of the tensor cores.
+//     That is 32768 FMAs a block and SM, 256 cycles of the fp32 pipes beside 512 of the tensor cores; what it costs is the
+//     way from the MMAs to the epilogue and back, which two accumulators hide only in part
+//     (12 x 4000 x 24576 x 768: 924 us, 696 with the next point).
+//   * So blocks that follow one another with the same scales, as most do where A's blocks are 128 x 128 (powers of two, of
+//     weights or gradients of one kind), are multiplied into one accumulator, up to kMostJoined of them (1024 products a sum).
 //   * MN-major operands come in boxes of 128(MN) x 128(K): K rows of 128 B, 8-row groups 1024 B apart, boxes 16 KB apart; the
 //     32-wide K step of one MMA moves the start address by 4096 B (K-major: by 32 B).
 //
@@ -35,8 +39,8 @@ using tc::kThreads;
 using tc::kTmemCols;
 constexpr int kBK = 128;         // contraction of a stage = of a scale block
 constexpr int kBox = 128 * 128;  // bytes of one box
-constexpr int kRegsLean = 56, kRegsEpi = 224;  // 128 * 56 + 256 * 224 = 384 * 168, what the block is launched with
-constexpr int kBatch = 8;        // blocks whose scales are handed to the epilogue together
+constexpr int kRegsLean = 88, kRegsEpi = 208;  // 128 * 88 + 256 * 208 = 384 * 168, what the block is launched with
+constexpr int kMostJoined = 8;   // blocks whose products may share one sum in tensor memory
 
 template <bool kPair>
 struct Tile {
@@ -53,16 +57,21 @@ static_assert(Tile<true>::kStages * Tile<true>::kStageBytes <= kOperandBytes &&
                   Tile<false>::kStages * Tile<false>::kStageBytes <= kOperandBytes,
               "operand stages");
 constexpr int kOutBytes = 8 * 1024;  // a warp's output on its way to memory: two boxes of 32 rows x 128 B
-// Scales of two batches, of the tile's 128 rows and of its two halves of the columns, and the bias of two tiles.
-struct ScaleRing {
-  float a[2][kBatch][128];
-  float b[2][kBatch][2];
-  float bias[2][kBN];
-  uint64_t full[2], empty[2];
+// Scales on their way to the epilogue, a window of blocks at a time.  Bit i of `starts`: block i begins a group, blocks with the same
+// scales that share one sum in tensor memory; `a` and `b` hold the groups' scales, of the tile's 128 rows (A in 1 x 128: every
+// block is a group) or of the whole tile, and of its two halves of columns.
+template <bool kByRow>
+struct alignas(16) ScaleRing {
+  static constexpr int kWindow = kByRow ? 8 : 32, kSlots = kByRow ? 2 : 4;
+  float a[kSlots][kByRow ? kWindow * 128 : kWindow];
+  float b[kSlots][kWindow][2];
+  float bias[kSlots][kBN];  // of tiles, which have a window each at least
+  uint32_t starts[kSlots];
+  uint64_t full[kSlots], empty[kSlots];
 };
 constexpr int kSmemBytes =
-    kOperandBytes + kEpiWarps * kOutBytes + 1024 /*alignment slack*/ + 256 /*barriers*/ + (int)sizeof(ScaleRing);
-static_assert(sizeof(tc::Barriers) <= 256 && sizeof(ScaleRing) % 16 == 0 && kSmemBytes <= 232448, "shared memory");
+    kOperandBytes + kEpiWarps * kOutBytes + 1024 /*alignment slack*/ + 256 /*barriers*/ + (int)sizeof(ScaleRing<true>);
+static_assert(sizeof(tc::Barriers) <= 256 && sizeof(ScaleRing<false>) <= sizeof(ScaleRing<true>) && kSmemBytes <= 232448, "shared memory");
 constexpr int kScaleWarps = 2;  // warps 2 and 3
 
 // Scales of one operand: element strides between matrices, between blocks along M (or N) and along K.
@@ -270,7 +279,7 @@ __device__ __forceinline__ void store_warp(float (&acc)[128], const float* bias,
   }
 }
 
-template <bool A_MN, bool B_MN, bool kPair, int kOut>
+template <bool A_MN, bool B_MN, bool kPair, int kOut, bool kByRow>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                 const __grid_constant__ CUtensorMap mapOut, GemmGeom g, Scales sa, Scales sb, Out out, int* status) {
@@ -280,7 +289,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* out_smem = smem + kOperandBytes;
   tc::Barriers* bars = reinterpret_cast<tc::Barriers*>(out_smem + kEpiWarps * kOutBytes);
-  ScaleRing* ring = reinterpret_cast<ScaleRing*>(out_smem + kEpiWarps * kOutBytes + 256);
+  using Ring = ScaleRing<kByRow>;
+  constexpr int kSlots = Ring::kSlots, window = Ring::kWindow;
+  Ring* ring = reinterpret_cast<Ring*>(out_smem + kEpiWarps * kOutBytes + 256);
   volatile int* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -303,9 +314,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
       tc::mbar_init(tc::smem_u32(&bars->tmem_full[i]), 1);
       tc::mbar_init(tc::smem_u32(&bars->tmem_empty[i]), TL::kCtas * kEpiWarps);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       tc::mbar_init(tc::smem_u32(&ring->full[i]), kScaleWarps);
-      tc::mbar_init(tc::smem_u32(&ring->empty[i]), kEpiWarps);
+      // the epilogue and, of the leader and where blocks are joined, the MMA warp
+      tc::mbar_init(tc::smem_u32(&ring->empty[i]), kEpiWarps + (rank == 0 && !kByRow ? 1 : 0));
     }
     bars->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -409,33 +421,48 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         constexpr int kStepA = (A_MN ? 4096 : 32) / 16, kStepB = (B_MN ? 4096 : 32) / 16;
         int stage = 0;
         uint32_t phase = 0;
-        uint32_t n = 0;  // blocks so far: accumulator n & 1, used for the (n >> 1)-th time
+        uint32_t n = 0, batch = 0;  // groups so far: accumulator n & 1, used for the (n >> 1)-th time; windows so far
         bool alive = true;
         for (int it = 0; alive; ++it) {
           const long long tile_l = tc::tile_of_round(it, worker, workers);
           if (tile_l >= total_tiles) break;
           int z, kb_lo, kb_hi, zo;
           work_item(g, (int)tile_l / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
-          for (int kb = kb_lo; kb < kb_hi; ++kb, ++n) {
-            const uint32_t buf = n & 1;
-            if (!wait(acc_empty0 + 8 * buf, ((n >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty) ||
-                !wait(full0 + 8 * stage, phase, abort_flag, status, kTimeoutFull)) {
-              alive = false;
-              break;
+          for (int left = kb_hi - kb_lo; left > 0 && alive; left -= window, ++batch) {
+            const int slot = batch % kSlots, in_window = min(left, window);
+            uint32_t starts = 0xffffffffu;
+            if constexpr (!kByRow) {
+              if (!wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutFull)) {
+                alive = false;
+                break;
+              }
+              starts = ring->starts[slot];
             }
-            __syncwarp();
-            tc::tc_fence_after();
-            if (one) {
-              const uint32_t tmem_d = tmem_base + buf * kBN;
-              const uint64_t da = da0 + (uint32_t)(stage * (kStageBytes / 16)), db = db0 + (uint32_t)(stage * (kStageBytes / 16));
+            for (int i = 0; i < in_window; ++i) {
+              const uint32_t buf = n & 1;
+              const bool first = starts >> i & 1, last = i + 1 == in_window || (starts >> (i + 1) & 1);
+              if ((first && !wait(acc_empty0 + 8 * buf, ((n >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty)) ||
+                  !wait(full0 + 8 * stage, phase, abort_flag, status, kTimeoutFull)) {
+                alive = false;
+                break;
+              }
+              __syncwarp();
+              tc::tc_fence_after();
+              if (one) {
+                const uint32_t tmem_d = tmem_base + buf * kBN;
+                const uint64_t da = da0 + (uint32_t)(stage * (kStageBytes / 16)), db = db0 + (uint32_t)(stage * (kStageBytes / 16));
 #pragma unroll
-              for (int k = 0; k < kBK / 32; ++k)
-                umma_e4m3<kPair>(tmem_d, da + k * kStepA, db + k * kStepB, idesc, k > 0 ? 1u : 0u);
-              tc::umma_commit<kPair>(empty0 + 8 * stage);
-              tc::umma_commit<kPair>(acc_full0 + 8 * buf);
+                for (int k = 0; k < kBK / 32; ++k)
+                  umma_e4m3<kPair>(tmem_d, da + k * kStepA, db + k * kStepB, idesc, k > 0 || !first ? 1u : 0u);
+                tc::umma_commit<kPair>(empty0 + 8 * stage);
+                if (last) tc::umma_commit<kPair>(acc_full0 + 8 * buf);
+              }
+              __syncwarp();
+              if (++stage == kStages) stage = 0, phase ^= 1;
+              if (last) ++n;
             }
             __syncwarp();
-            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (lane == 0 && !kByRow) tc::mbar_arrive(tc::smem_u32(&ring->empty[slot]));
           }
           alive = __all_sync(0xffffffffu, alive);
         }
@@ -453,46 +480,81 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         int z, kb_lo, kb_hi, zo, m0, n0;
         work_item(g, tile / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
         tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
-        m0 += rank * kBM;
-        // rows and columns behind the end take the last one's: their sums are not stored
-        const float* a0 = sa.p + (long long)(min(m0 + t, g.M - 1) >> sa.shift) * sa.mn;
-        const float* a1 = sa.p + (long long)(min(m0 + t + 64, g.M - 1) >> sa.shift) * sa.mn;
-        const float* b0 = sb.p + (long long)(min(n0 + 128 * (t & 1), g.N - 1) >> 7) * sb.mn;
-        int j = kb_lo / kb_per_seg, kb = kb_lo % kb_per_seg;
-        int za, zb;
-        seg_index(g, z, j, za, zb);
-        for (int left = kb_hi - kb_lo; left > 0; left -= kBatch, ++batch) {
-          const int slot = batch & 1;
+        // rows and columns behind the end take the last ones' scales: their sums are not stored
+        const auto row_of = [&](int m) { return sa.p + (long long)(min(m, g.M - 1) >> sa.shift) * sa.mn; };
+        const float* b0 = sb.p + (long long)(min(n0, g.N - 1) >> 7) * sb.mn;
+        const float* b1 = sb.p + (long long)(min(n0 + 128, g.N - 1) >> 7) * sb.mn;
+        // by row: this thread's rows t and t + 64 of the CTA's and a half of the columns, from block `at` on
+        const float *pa0 = nullptr, *pa1 = nullptr, *pb = nullptr;
+        int seg_left = 0;
+        const auto segment = [&](int at) {
+          const int j = at / kb_per_seg, kb = at - j * kb_per_seg;
+          int za, zb;
+          seg_index(g, z, j, za, zb);
+          const long long oa = za * sa.z + kb * sa.k;
+          pa0 = row_of(m0 + rank * kBM + t) + oa, pa1 = row_of(m0 + rank * kBM + t + 64) + oa;
+          pb = (t & 1 ? b1 : b0) + zb * sb.z + kb * sb.k;
+          seg_left = kb_per_seg - kb;
+        };
+        for (int at = kb_lo; at < kb_hi; at += window, ++batch) {
+          const int slot = batch % kSlots, n = min(kb_hi - at, window);
           const bool ok =
-              wait(tc::smem_u32(&ring->empty[slot]), ((batch >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty);
+              wait(tc::smem_u32(&ring->empty[slot]), ((batch / kSlots) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty);
           alive = __all_sync(0xffffffffu, ok);
           if (!alive) break;
-          const int n = min(left, kBatch);
-          if (out.bias != nullptr && left == kb_hi - kb_lo) {
-            // with the tile's first batch; the tile before last has given its last batch back, which it does after its output
+          if (out.bias != nullptr && at == kb_lo) {
+            // with the tile's first window, once the tile kSlots before has been put out
 #pragma unroll
             for (int i = 0; i < kBN; i += 64)
-              ring->bias[it & 1][i + t] = n0 + i + t < g.N ? __ldg(out.bias + zo * out.bias_z + n0 + i + t) : 0.f;
+              ring->bias[it % kSlots][i + t] = n0 + i + t < g.N ? __ldg(out.bias + zo * out.bias_z + n0 + i + t) : 0.f;
           }
-          float va[kBatch], vb[kBatch], vc[kBatch];
+          if constexpr (kByRow) {
+            float va[window], vb[window], vc[window];
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            if (i < n) {
-              const long long oa = za * sa.z + kb * sa.k;
-              va[i] = __ldg(a0 + oa), vb[i] = __ldg(a1 + oa);
-              vc[i] = t < 2 ? __ldg(b0 + zb * sb.z + kb * sb.k) : 0.f;
-              if (++kb == kb_per_seg) {
-                kb = 0, ++j;
-                if (i + 1 < left) seg_index(g, z, j, za, zb);
+            for (int i = 0; i < window; ++i) {
+              if (i < n) {
+                if (seg_left == 0) segment(at + i);
+                va[i] = __ldg(pa0), vb[i] = __ldg(pa1);
+                vc[i] = t < 2 ? __ldg(pb) : 0.f;
+                pa0 += sa.k, pa1 += sa.k, pb += sb.k, --seg_left;
               }
             }
-          }
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            if (i < n) {
-              ring->a[slot][i][t] = va[i], ring->a[slot][i][t + 64] = vb[i];
-              if (t < 2) ring->b[slot][i][t] = vc[i];
+            for (int i = 0; i < window; ++i) {
+              if (i < n) {
+                ring->a[slot][i * 128 + t] = va[i], ring->a[slot][i * 128 + t + 64] = vb[i];
+                if (t < 2) ring->b[slot][i][t] = vc[i];
+              }
             }
+          } else if (warp == 2) {
+            // lane i has block at + i: its scales of both CTAs' rows and of both halves of the columns
+            float v[4] = {};
+            if (lane < n) {
+              const int j = (at + lane) / kb_per_seg, kb = at + lane - j * kb_per_seg;
+              int za, zb;
+              seg_index(g, z, j, za, zb);
+              v[0] = __ldg(row_of(m0) + za * sa.z + kb * sa.k);
+              v[1] = kPair ? __ldg(row_of(m0 + kBM) + za * sa.z + kb * sa.k) : v[0];
+              v[2] = __ldg(b0 + zb * sb.z + kb * sb.k);
+              v[3] = __ldg(b1 + zb * sb.z + kb * sb.k);
+            }
+            bool differs = lane == 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) differs |= !(v[i] == __shfl_up_sync(0xffffffffu, v[i], 1));
+            const uint32_t changes = __ballot_sync(0xffffffffu, differs && lane < n);
+            uint32_t starts = 0;
+            for (int p = 0; p < n;) {
+              starts |= 1u << p;
+              const uint32_t later = changes & ~((2u << p) - 1);
+              const int next = later != 0 ? __ffs(later) - 1 : n;
+              p = min(next, p + kMostJoined);
+            }
+            if (starts >> lane & 1) {
+              const int group = __popc(starts & ((1u << lane) - 1));
+              ring->a[slot][group] = rank == 0 ? v[0] : v[1];
+              ring->b[slot][group][0] = v[2], ring->b[slot][group][1] = v[3];
+            }
+            if (lane == 0) ring->starts[slot] = starts;
           }
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->full[slot]));
@@ -528,16 +590,16 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
       alive = block_ready(bars, n, abort_flag, status);
       if (alive && work) tmem_ld16_issue(tbase + (n & 1) * kBN, r0);
 #pragma unroll 1
-      for (int left = kb_hi - kb_lo; left > 0 && alive; left -= kBatch, ++batch) {
-        const int slot = batch & 1;
-        alive = wait(tc::smem_u32(&ring->full[slot]), (batch >> 1) & 1, abort_flag, status, kTimeoutTmemFull);
+      for (int left = kb_hi - kb_lo; left > 0 && alive; left -= window, ++batch) {
+        const int slot = batch % kSlots;
+        alive = wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutTmemFull);
         alive = __all_sync(0xffffffffu, alive);
-        const float* ra = &ring->a[slot][0][quarter * 32 + lane];
+        const float* ra = ring->a[slot] + (kByRow ? quarter * 32 + lane : 0);
         const float* rb = &ring->b[slot][0][half];
-        const int in_batch = min(left, kBatch);
+        const int groups = kByRow ? min(left, window) : __popc(ring->starts[slot]);
 #pragma unroll 1
-        for (int i = 0; alive && i < in_batch; ++i, ++n) {
-          const float s = ra[i * 128] * rb[i * 2];
+        for (int i = 0; alive && i < groups; ++i, ++n) {
+          const float s = ra[kByRow ? i * 128 : i] * rb[i * 2];
           const int buf = n & 1;
           const uint32_t taddr = tbase + buf * kBN;
           if (work) {
@@ -561,14 +623,14 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             else
               tc::mbar_arrive(tc::smem_u32(&bars->tmem_empty[buf]));
           }
-          if (i + 1 < left) {
+          if (i + 1 < groups || left > window) {
             alive = block_ready(bars, n + 1, abort_flag, status);
             if (alive && work) tmem_ld16_issue(tbase + ((n + 1) & 1) * kBN, r0);
           }
           if (work) fma16(acc + 112, r1, s);
         }
-        if (left <= kBatch && alive && work)  // before the slot is given back: the bias that it brought is read here
-          store_warp<kOut>(acc, ring->bias[it & 1] + half * 128, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);
+        if (left <= window && alive && work)  // before the slot is given back: the bias that it brought is read here
+          store_warp<kOut>(acc, ring->bias[it % kSlots] + half * 128, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->empty[slot]));
       }
