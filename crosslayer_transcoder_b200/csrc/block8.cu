@@ -32,10 +32,26 @@ struct Vec8<float> {
     a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
   }
   __device__ __forceinline__ void store(float* p) const { st_cs8(p, a, b); }
+  // The largest magnitude so far, as bits: they are ordered as the magnitudes are, infinities and NaN behind all numbers.
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
+  static constexpr uint32_t kInf = 0x7f800000u;
+  static __device__ __forceinline__ uint32_t join(uint32_t m) { return m; }
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __uint_as_float(bits); }
 };
 template <class T>
 struct Vec8Half {
   uint4 a;
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    return m;
+  }
   __device__ __forceinline__ void load(const T* p) { a = __ldcs(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), a); }
 };
@@ -49,6 +65,9 @@ struct Vec8<__nv_bfloat16> : Vec8Half<__nv_bfloat16> {
   __device__ __forceinline__ void put(const float (&v)[8]) {
     a = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
   }
+  static constexpr uint32_t kInf = 0x7f80u;
+  static __device__ __forceinline__ uint32_t join(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __uint_as_float(bits << 16); }
 };
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -67,6 +86,9 @@ struct Vec8<__half> : Vec8Half<__half> {
   __device__ __forceinline__ void put(const float (&v)[8]) {
     a = make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
   }
+  static constexpr uint32_t kInf = 0x7c00u;
+  static __device__ __forceinline__ uint32_t join(uint32_t m) { return max(m & 0xffffu, m >> 16); }
+  static __device__ __forceinline__ float magnitude(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
 };
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -122,17 +144,20 @@ __device__ __forceinline__ float inverse_scale(float s) { return __uint_as_float
 
 __device__ __forceinline__ float not_inf(float v) { return fabsf(v) <= 3.402823466e38f ? v : __uint_as_float(0x7fffffffu); }
 
-__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv) {
+// `all`: some of the block's values are not finite (the conversion takes infinities for large numbers)
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8], float inv, bool all) {
   uint32_t h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(not_inf(v[2 * i]) * inv, not_inf(v[2 * i + 1]) * inv), __NV_SATFINITE, __NV_E4M3);
+    h[i] = __nv_cvt_float2_to_fp8x2(make_float2((all ? not_inf(v[2 * i]) : v[2 * i]) * inv,
+                                                (all ? not_inf(v[2 * i + 1]) : v[2 * i + 1]) * inv),
+                                    __NV_SATFINITE, __NV_E4M3);
   return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
 }
 
-__device__ __forceinline__ float max16(float v) {  // over groups of 16 lanes
+__device__ __forceinline__ uint32_t max16(uint32_t v) {  // over groups of 16 lanes
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 
@@ -144,58 +169,83 @@ struct Source {
 };
 
 // One CTA per 128 x 128 block, 16 lanes x 8 values to a row, 8 rows to a thread: the block is read once, all of it at a time.
-// sums (may be NULL): sums[z, block of rows, c] = the block's column sums (of what came in), for bias gradients.
-template <class T>
+// Magnitudes are compared as integers, two 16-bit ones at a time; where a block turns out to hold infinities or NaN they are
+// found again without those.
+// kSums: sums[z, block of rows, c] = the block's column sums (of what came in), for bias gradients.
+template <class T, bool kSums>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(Source s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
                                                             float* __restrict__ sums, int row_blocks, int col_blocks) {
-  __shared__ float part[8];
-  __shared__ float colsum[16][128];
+  using V = Vec8<T>;
+  __shared__ uint32_t part[2][8];
   const int cb = blockIdx.x % col_blocks, rb = blockIdx.x / col_blocks, z = blockIdx.y;
   const int g = threadIdx.x >> 4, c = cb * 128 + (threadIdx.x & 15) * 8;
   const int n = s.C - c;
   const bool vec = s.vec && n >= 8;
   const T* x = (const T*)s.x + z * s.z + (long long)(rb * 128 + g) * s.ld + c;
   const int rows = s.R - rb * 128 - g;
-  Vec8<T> v[8];
+  V v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = load8<T>(x + (long long)(16 * i) * s.ld, 16 * i < rows ? n : 0, vec && 16 * i < rows);
-  float amax = 0.f, f[8];
-  float cs[8] = {};
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i].get(f);
+  for (int i = 0; i < 8; ++i) top = v[i].top(top);
+  top = max16(V::join(top));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+  if ((threadIdx.x & 31) == 0) part[0][threadIdx.x >> 5] = top;
+  if constexpr (kSums) {
+    __shared__ float colsum[16][128];
+    float cs[8] = {}, f[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, finite_abs(f[k]));
-    if (sums != nullptr) {
+    for (int i = 0; i < 8; ++i) {
+      v[i].get(f);
 #pragma unroll
       for (int k = 0; k < 8; ++k) cs[k] += f[k];
     }
-  }
-  amax = max16(amax);
-  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
-  if (sums != nullptr) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) colsum[g][(threadIdx.x & 15) * 8 + k] = cs[k];
-  }
-  __syncthreads();
+    for (int k = 0; k < 8; k += 4)
+      *reinterpret_cast<float4*>(&colsum[g][(threadIdx.x & 15) * 8 + k]) = make_float4(cs[k], cs[k + 1], cs[k + 2], cs[k + 3]);
+    __syncthreads();
+    if (threadIdx.x < 128 && cb * 128 + threadIdx.x < s.C) {
+      float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, part[i]);
+      for (int i = 0; i < 16; ++i) t += colsum[i][threadIdx.x];
+      sums[((long long)z * row_blocks + rb) * s.C + cb * 128 + threadIdx.x] = t;
+    }
+  } else {
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, part[0][i]);
+  const bool all = top >= V::kInf;  // uniform over the CTA
+  float amax = V::magnitude(top);
+  if (all) {
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float f[8];
+      v[i].get(f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, finite_abs(f[k]));
+    }
+    uint32_t bits = max16(__float_as_uint(amax));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, 16));
+    if ((threadIdx.x & 31) == 0) part[1][threadIdx.x >> 5] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bits = max(bits, part[1][i]);
+    amax = __uint_as_float(bits);
+  }
   const float scale = block_scale(amax), inv = inverse_scale(scale);
   if (threadIdx.x == 0) scales[((long long)z * row_blocks + rb) * col_blocks + cb] = scale;
   uint8_t* out = q + ((long long)z * s.R + rb * 128 + g) * q_ld + c;
+  if (c >= q_ld) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (16 * i < rows && c < q_ld) {
+    if (16 * i < rows) {
+      float f[8];
       v[i].get(f);
-      *reinterpret_cast<uint2*>(out + (long long)(16 * i) * q_ld) = to_e4m3x8(f, inv);
+      *reinterpret_cast<uint2*>(out + (long long)(16 * i) * q_ld) = to_e4m3x8(f, inv, all);
     }
-  }
-  if (sums != nullptr && threadIdx.x < 128 && cb * 128 + threadIdx.x < s.C) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t += colsum[i][threadIdx.x];
-    sums[((long long)z * row_blocks + rb) * s.C + cb * 128 + threadIdx.x] = t;
   }
 }
 
@@ -203,32 +253,41 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(Source s, uint8_t* _
 constexpr int kAhead = 4;
 template <class T>
 __global__ void __launch_bounds__(256) quantize_row_kernel(Source s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
-                                                           int col_blocks, long long blocks) {
+                                                           int col_blocks, unsigned blocks) {
+  using V = Vec8<T>;
   const int lane = threadIdx.x & 15;
-  const long long first = ((long long)blockIdx.x * 16 + (threadIdx.x >> 4)) * kAhead;
-  Vec8<T> v[kAhead];
-  long long row[kAhead];
-  int c[kAhead];
+  const unsigned first = (blockIdx.x * 16 + (threadIdx.x >> 4)) * kAhead;
+  V v[kAhead];
+  unsigned row = first / col_blocks, cb = first - row * col_blocks;
+  unsigned z = row / s.R, r = row - z * s.R;
+  long long to[kAhead];  // where the copy goes, -1: nowhere
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    const long long b = first + i;
-    row[i] = b / col_blocks;
-    c[i] = (int)(b - row[i] * col_blocks) * 128 + lane * 8;
-    const long long z = row[i] / s.R, r = row[i] - z * s.R;
-    const int n = b < blocks ? s.C - c[i] : 0;
-    v[i] = load8<T>((const T*)s.x + z * s.z + r * s.ld + c[i], n, s.vec && n >= 8);
+    const int c = (int)cb * 128 + lane * 8, n = first + i < blocks ? s.C - c : 0;
+    v[i] = load8<T>((const T*)s.x + z * s.z + r * s.ld + c, n, s.vec && n >= 8);
+    to[i] = first + i < blocks && c < q_ld ? (long long)row * q_ld + c : -1;
+    if (++cb == (unsigned)col_blocks) {
+      cb = 0, ++row;
+      if (++r == (unsigned)s.R) r = 0, ++z;
+    }
   }
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
-    float f[8], amax = 0.f;
+    float f[8];
     v[i].get(f);
+    const uint32_t top = max16(V::join(v[i].top(0)));
+    const bool all = top >= V::kInf;
+    float amax = V::magnitude(top);
+    if (__any_sync(0xffffffffu, all)) {
+      float a = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, finite_abs(f[k]));
-    const float scale = block_scale(max16(amax));
-    if (first + i < blocks) {
-      if (lane == 0) scales[first + i] = scale;
-      if (c[i] < q_ld) *reinterpret_cast<uint2*>(q + row[i] * q_ld + c[i]) = to_e4m3x8(f, inverse_scale(scale));
+      for (int k = 0; k < 8; ++k) a = fmaxf(a, finite_abs(f[k]));
+      a = __uint_as_float(max16(__float_as_uint(a)));
+      if (all) amax = a;
     }
+    const float scale = block_scale(amax);
+    if (first + i < blocks && lane == 0) scales[first + i] = scale;
+    if (to[i] >= 0) *reinterpret_cast<uint2*>(q + to[i]) = to_e4m3x8(f, inverse_scale(scale), all);
   }
 }
 
@@ -294,10 +353,11 @@ __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict
 }
 
 // ---- (Jump)ReLU with a two-bit checkpoint ---------------------------------------------------------------
-// A thread has 8 columns with their thresholds and walks down the rows, two of them in flight.  A word of the checkpoint is 16 bits for 8
+// A thread has 8 columns with their thresholds and walks down the rows, kRowsAhead of them in flight.  A word of the checkpoint is 16 bits for 8
 // values: the low byte has bit i where the gradient passes (x >= 0; ReLU: x > 0), the high byte where theta - bw/2 < x <= theta + bw/2,
 // the window in which the threshold gets a gradient.  Both bounds are rounded down from 64 bits, which decides the comparisons with
 // an fp32 x as the exact bounds would.
+constexpr int kRowsAhead = 4;
 struct Window {
   float lo[8], hi[8], theta[8];
 };
@@ -306,7 +366,7 @@ __device__ __forceinline__ void load_window(Window& w, const float* theta, Bandw
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float t = k < n ? theta[c + k] : 0.f;
-    w.theta[k] = t;
+    w.theta[k] = t != t ? __uint_as_float(0x7f800000u) : fmaxf(t, 0.f);  // x > theta and x > 0; nothing is above a NaN
     w.lo[k] = __double2float_rd((double)t - half);
     w.hi[k] = __double2float_rd((double)t + half);
   }
@@ -314,9 +374,8 @@ __device__ __forceinline__ void load_window(Window& w, const float* theta, Bandw
 
 template <class T, bool kJump>
 __global__ void __launch_bounds__(256) jump_relu_fwd_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ theta,
-                                                            Bandwidth bandwidth, T* __restrict__ y,
-                                                            uint16_t* __restrict__ bits, int R, int C, int rows_per_cta, int in_vec,
-                                                            int out_vec) {
+                                                            Bandwidth bandwidth, T* __restrict__ y, uint16_t* __restrict__ bits,
+                                                            int R, int C, int rows_per_cta, int in_vec, int out_vec) {
   const int words = (C + 7) / 8, w = blockIdx.x * 256 + threadIdx.x;
   if (w >= words) return;
   const int c = w * 8, n = C - c;
@@ -324,26 +383,32 @@ __global__ void __launch_bounds__(256) jump_relu_fwd_kernel(const T* __restrict_
   if constexpr (kJump) load_window(win, theta, bandwidth, c, n);
   const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
   const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
-#pragma unroll 2
-  for (int r = r0; r < r1; ++r) {
-    const Vec8<T> v = load8<T>(x + r * ld + c, n, iv);
-    float f[8];
-    v.get(f);
-    uint32_t m = 0;
+  for (int r = r0; r < r1; r += kRowsAhead) {
+    Vec8<T> v[kRowsAhead];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float t = f[k];
-      if constexpr (kJump) {
-        m |= (t < 0.f ? 0u : 1u) << k;
-        m |= (t > win.lo[k] && t <= win.hi[k] ? 256u : 0u) << k;
-        f[k] = (t <= win.theta[k] || t <= 0.f) ? 0.f : t;  // NaN stays
-      } else {
-        m |= (t <= 0.f ? 0u : 1u) << k;
-        f[k] = t <= 0.f ? 0.f : t;
+    for (int i = 0; i < kRowsAhead; ++i) v[i] = load8<T>(x + (r + i) * ld + c, r + i < r1 ? n : 0, iv && r + i < r1);
+#pragma unroll
+    for (int i = 0; i < kRowsAhead; ++i) {
+      if (r + i < r1) {
+        float f[8];
+        v[i].get(f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = f[k];
+          if constexpr (kJump) {
+            if (!(t < 0.f)) m |= 1u << k;
+            if (t > win.lo[k] && t <= win.hi[k]) m |= 256u << k;
+            f[k] = t <= win.theta[k] ? 0.f : t;  // (at least 0; NaN stays)
+          } else {
+            if (!(t <= 0.f)) m |= 1u << k;
+            f[k] = t <= 0.f ? 0.f : t;
+          }
+        }
+        store8<T>(y + (long long)(r + i) * C + c, n, ov, f);
+        bits[(long long)(r + i) * words + w] = (uint16_t)m;
       }
     }
-    store8<T>(y + (long long)r * C + c, n, ov, f);
-    bits[(long long)r * words + w] = (uint16_t)m;
   }
 }
 
@@ -357,18 +422,27 @@ __global__ void __launch_bounds__(256) jump_relu_bwd_kernel(const T* __restrict_
   const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
   const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
   float acc[8] = {};
-#pragma unroll 4
-  for (int r = r0; r < r1; ++r) {
-    const Vec8<T> v = load8<T>(g + r * ld + c, n, iv);
-    const uint32_t m = bits[(long long)r * words + w];
-    float f[8];
-    v.get(f);
+  for (int r = r0; r < r1; r += kRowsAhead) {
+    Vec8<T> v[kRowsAhead];
+    uint32_t m[kRowsAhead];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (kJump && (m >> (8 + k) & 1)) acc[k] += f[k];
-      if (!(m >> k & 1)) f[k] = 0.f;
+    for (int i = 0; i < kRowsAhead; ++i) {
+      v[i] = load8<T>(g + (r + i) * ld + c, r + i < r1 ? n : 0, iv && r + i < r1);
+      m[i] = r + i < r1 ? bits[(long long)(r + i) * words + w] : 0u;
     }
-    store8<T>(dx + (long long)r * C + c, n, ov, f);
+#pragma unroll
+    for (int i = 0; i < kRowsAhead; ++i) {
+      if (r + i < r1) {
+        float f[8];
+        v[i].get(f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (kJump && (m[i] & (256u << k))) acc[k] += f[k];
+          if (!(m[i] & (1u << k))) f[k] = 0.f;
+        }
+        store8<T>(dx + (long long)(r + i) * C + c, n, ov, f);
+      }
+    }
   }
   if constexpr (kJump) {
 #pragma unroll
@@ -392,13 +466,17 @@ template <class T>
 int quantize(const Source& s, uint8_t* q, int q_ld, float* scales, float* sums, int Z, int block_rows, cudaStream_t st) {
   const int cb = (int)up(s.C, 128);
   if (block_rows == 1) {
-    const long long blocks = (long long)Z * s.R * cb, grid = up(blocks, 16 * kAhead);
-    CLT_CHECK_ARG(grid < (1ll << 31), "fp8_quantize: too many blocks");
-    quantize_row_kernel<T><<<(unsigned)grid, 256, 0, st>>>(s, q, q_ld, scales, cb, blocks);
+    const long long blocks = (long long)Z * s.R * cb;
+    CLT_CHECK_ARG(blocks < (1ll << 31), "fp8_quantize: too many blocks");
+    quantize_row_kernel<T><<<(unsigned)up(blocks, 16 * kAhead), 256, 0, st>>>(s, q, q_ld, scales, cb, (unsigned)blocks);
   } else {
     const long long rb = up(s.R, 128);
     CLT_CHECK_ARG(rb * cb < (1ll << 31) && Z <= 65535, "fp8_quantize: too many blocks");
-    quantize_tile_kernel<T><<<dim3((unsigned)(rb * cb), Z), 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
+    const dim3 grid((unsigned)(rb * cb), Z);
+    if (sums != nullptr)
+      quantize_tile_kernel<T, true><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
+    else
+      quantize_tile_kernel<T, false><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
   }
   CLT_CHECK_CUDA(cudaGetLastError());
   return 0;

@@ -68,42 +68,40 @@ def check_status(where: str = ""):
             _raise_status(where)
 
 
-def _need(cond: bool, text: str):
-    if not cond:
-        raise ValueError(text)
-
-
-def _check(name: str, t, dtypes=None, device=None):
+def _check(name: str, t, dtypes, device=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has type {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if dtypes is not None and t.dtype not in dtypes:
-        raise TypeError(f"{name} has type {t.dtype}, expected one of {', '.join(str(d) for d in dtypes)}")
 
 
-class _On:
-    """The device of the operands as the current one."""
+_checked = set()
 
-    def __init__(self, device):
-        if device.type != "cuda":
-            raise CltError(f"the 8-bit operators run on CUDA tensors only (no CPU fallback), got {device}")
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        lib().check_device()
+def _on(device, fn, *args):
+    """``fn(*args)`` with the operands' device as the current one."""
+    if device.type != "cuda":
+        raise CltError(f"the 8-bit operators run on CUDA tensors only (no CPU fallback), got {device}")
+    if torch.cuda.is_initialized() and torch._C._cuda_getDevice() == device.index:
+        if device.index not in _checked:
+            lib().check_device()
+            _checked.add(device.index)
+        return fn(*args)
+    with torch.cuda.device(device):
+        return _on(device, fn, *args)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _pitch(C: int) -> int:
+    return (C + 15) & ~15
 
 
 def _storage(*shape, device):
     """8-bit values [..., C] whose rows start on 16 bytes."""
-    pitch = -(-shape[-1] // 16) * 16
-    return torch.empty(*shape[:-1], pitch, dtype=torch.float8_e4m3fn, device=device)[..., :shape[-1]]
+    C = shape[-1]
+    v = torch.empty(*shape[:-1], _pitch(C), dtype=torch.float8_e4m3fn, device=device)
+    return v if C % 16 == 0 else v[..., :C]
 
 
 class BlockTensor:
@@ -116,11 +114,21 @@ class BlockTensor:
     def __init__(self, values: torch.Tensor, scales: torch.Tensor, block_rows: int = BLOCK):
         _check("values", values, (torch.float8_e4m3fn,))
         _check("scales", scales, (torch.float32,), values.device)
-        _need(block_rows in (1, BLOCK), f"blocks of {block_rows} rows: 1 or 128 are supported")
-        _need(values.dim() in (2, 3), f"expected a matrix or a stack of matrices, got {tuple(values.shape)}")
-        want = (*values.shape[:-2], _blocks(values.shape[-2], block_rows), _blocks(values.shape[-1]))
-        _need(tuple(scales.shape) == want, f"scales {tuple(scales.shape)} do not match {want}")
+        if block_rows not in (1, BLOCK):
+            raise ValueError(f"blocks of {block_rows} rows: 1 or 128 are supported")
+        shape = values.shape
+        if len(shape) not in (2, 3):
+            raise ValueError(f"expected a matrix or a stack of matrices, got {tuple(shape)}")
+        want = (*shape[:-2], _blocks(shape[-2], block_rows), _blocks(shape[-1]))
+        if scales.shape != want:
+            raise ValueError(f"scales {tuple(scales.shape)} do not match {want}")
         self.values, self.scales, self.block_rows, self.transposed = values, scales, block_rows, False
+
+    @classmethod
+    def _of(cls, values, scales, block_rows, transposed=False):
+        t = object.__new__(cls)
+        t.values, t.scales, t.block_rows, t.transposed = values, scales, block_rows, transposed
+        return t
 
     @property
     def shape(self) -> torch.Size:
@@ -134,56 +142,59 @@ class BlockTensor:
     @property
     def mT(self) -> "BlockTensor":
         """The transposed matrices, without a copy."""
-        t = BlockTensor(self.values, self.scales, self.block_rows)
-        t.transposed = not self.transposed
-        return t
+        return self._of(self.values, self.scales, self.block_rows, not self.transposed)
 
     def __getitem__(self, i: int) -> "BlockTensor":
-        _need(self.values.dim() == 3, "only a stack of matrices is indexed")
-        t = BlockTensor(self.values[i], self.scales[i], self.block_rows)
-        t.transposed = self.transposed
-        return t
+        if self.values.dim() != 3 or not isinstance(i, int):
+            raise ValueError("a stack of matrices is indexed with one integer")
+        return self._of(self.values[i], self.scales[i], self.block_rows, self.transposed)
 
     def __repr__(self):
         return f"BlockTensor(shape={tuple(self.shape)}, block_rows={self.block_rows}, device={self.device})"
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """What the elements stand for, rounded once to ``dtype`` (fp32, fp16 or bf16)."""
-        _need(dtype in DTYPE_CODE, f"dequantize to fp32, fp16 or bf16, not {dtype}")
-        v, s = self._stack()
-        Z, R, C = v.shape
-        with _On(self.device):
-            out = torch.empty(Z, R, C, dtype=dtype, device=self.device)
-            if out.numel():
-                if v.stride(2) != 1:
-                    v = v.contiguous()
-                lib().call("clt_fp8_dequantize", v, v.stride(1), v.stride(0), s, *s.stride(), self.block_rows, out,
-                           DTYPE_CODE[dtype], Z, R, C, stream_ptr())
-        out = out.view(self.values.shape)
+        if dtype not in DTYPE_CODE:
+            raise ValueError(f"dequantize to fp32, fp16 or bf16, not {dtype}")
+        out = _on(self.device, _dequantize, self.values, self.scales, self.block_rows, dtype)
         return out.mT if self.transposed else out
 
-    def _stack(self):
-        v, s = self.values, self.scales
-        return (v, s) if v.dim() == 3 else (v.unsqueeze(0), s.unsqueeze(0))
+
+def _dequantize(v, s, block_rows, dtype):
+    out = torch.empty(v.shape, dtype=dtype, device=v.device)
+    if out.numel():
+        if v.stride(-1) != 1:
+            v = v.contiguous()
+        Z, v_z, s_z = (v.shape[0], v.stride(0), s.stride(0)) if v.dim() == 3 else (1, 0, 0)
+        R, C = v.shape[-2:]
+        lib().call("clt_fp8_dequantize", v, v.stride(-2), v_z, s, s_z, s.stride(-2), s.stride(-1), block_rows, out,
+                   DTYPE_CODE[dtype], Z, R, C, stream_ptr())
+    return out
 
 
-def _quantize(x: torch.Tensor, block_rows: int, sums: bool = False, into=None):
-    """(values, scales, column sums of x or None) of x [Z, R, C]; ``into``: (values, scales) to write to."""
-    if x.stride(2) != 1 and x.shape[2] > 1:
+def _quantize(x, x_ld: int, x_z: int, Z: int, R: int, C: int, block_rows: int, v, s, sums=None):
+    """x (rows x_ld apart, matrices x_z) to the values v [Z, R, pitch] and scales s; ``sums [Z, C]``: its column sums."""
+    if Z * R * C == 0:
+        if sums is not None:
+            sums.zero_()
+        return
+    part = None if sums is None else torch.empty(Z, _blocks(R), C, dtype=torch.float32, device=x.device)
+    lib().call("clt_fp8_quantize", x, DTYPE_CODE[x.dtype], x_ld, x_z, v, _pitch(C), s, part, Z, R, C, block_rows, stream_ptr())
+    if part is not None:
+        lib().call("clt_sum_chunks", part, sums, Z, _blocks(R), C, stream_ptr())
+
+
+def _quantize_any(x, block_rows):
+    """quantize of a matrix or a stack."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
         x = x.contiguous()
-    Z, R, C = x.shape
-    v, s = into or (_storage(Z, R, C, device=x.device),
-                    torch.empty(Z, _blocks(R, block_rows), _blocks(C), dtype=torch.float32, device=x.device))
-    part = torch.empty(Z, _blocks(R), C, dtype=torch.float32, device=x.device) if sums else None
-    total = torch.empty(Z, C, dtype=torch.float32, device=x.device) if sums else None
-    if x.numel():
-        lib().call("clt_fp8_quantize", x, DTYPE_CODE[x.dtype], x.stride(1), x.stride(0), v, v.stride(1), s, part, Z, R, C,
-                   block_rows, stream_ptr())
-        if sums:
-            lib().call("clt_sum_chunks", part, total, Z, _blocks(R), C, stream_ptr())
-    elif sums:
-        total.zero_()
-    return v, s, total
+    shape = x.shape
+    R, C = shape[-2:]
+    Z, x_z = (shape[0], x.stride(0)) if len(shape) == 3 else (1, 0)
+    v = _storage(*shape, device=x.device)
+    s = torch.empty(*shape[:-2], _blocks(R, block_rows), _blocks(C), dtype=torch.float32, device=x.device)
+    _quantize(x, x.stride(-2), x_z, Z, R, C, block_rows, v, s)
+    return BlockTensor._of(v, s, block_rows)
 
 
 def quantize(x: torch.Tensor, block_rows: int = BLOCK) -> BlockTensor:
@@ -191,44 +202,62 @@ def quantize(x: torch.Tensor, block_rows: int = BLOCK) -> BlockTensor:
     that brings its largest finite magnitude to at most 448, the largest e4m3 value; 1 for a block of zeros.  Elements are rounded
     to nearest; what is not finite becomes NaN and does not count for the scale."""
     _check("x", x, DTYPE_CODE)
-    _need(x.dim() in (2, 3), f"expected a matrix or a stack of matrices, got {tuple(x.shape)}")
-    _need(block_rows in (1, BLOCK), f"blocks of {block_rows} rows: 1 or 128 are supported")
-    x = x.detach()
-    with _On(x.device):
-        v, s, _ = _quantize(x if x.dim() == 3 else x.unsqueeze(0), block_rows)
-    return BlockTensor(v, s, block_rows) if x.dim() == 3 else BlockTensor(v[0], s[0], block_rows)
+    if x.dim() not in (2, 3):
+        raise ValueError(f"expected a matrix or a stack of matrices, got {tuple(x.shape)}")
+    if block_rows not in (1, BLOCK):
+        raise ValueError(f"blocks of {block_rows} rows: 1 or 128 are supported")
+    return _on(x.device, _quantize_any, x.detach(), block_rows)
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------------
-def _aligned(v: torch.Tensor) -> torch.Tensor:
-    """``v [Z, R, C]``, copied where the tensor-core path cannot read it in place: rows have to start on 16 bytes."""
-    Z, R, C = v.shape
-    if (v.stride(2) == 1 or C == 1) and v.data_ptr() % 16 == 0 and (R == 1 or (v.stride(1) % 16 == 0 and v.stride(1) >= C)) and \
-            (Z == 1 or (v.stride(0) % 16 == 0 and v.stride(0) > 0)):
-        return v
-    out = _storage(Z, R, C, device=v.device)
-    out.view(torch.uint8).copy_(v.view(torch.uint8))
-    return out
+def _operand(v: torch.Tensor, s: torch.Tensor, rows_are_k: bool, transposed: bool):
+    """What ``clt_fp8_matmul`` takes of an operand: values, distances of rows and matrices, whether it is stored transposed, scales and
+    their distances between matrices, along M or N and along K.  Copied where the tensor-core path cannot read the values in place:
+    rows have to start on 16 bytes."""
+    stack = v.dim() == 3
+    Z, z = (v.shape[0], v.stride(0)) if stack else (1, 0)
+    R, C = v.shape[-2:]
+    ld = v.stride(-2)
+    if R == 1:
+        ld = _pitch(C)
+    if (v.stride(-1) != 1 and C > 1) or ld % 16 or ld < C or v.data_ptr() % 16 or (Z > 1 and (z % 16 or z <= 0)):
+        copy = _storage(*v.shape, device=v.device)
+        copy.view(torch.uint8).copy_(v.view(torch.uint8))
+        v, ld, z = copy, _pitch(C), R * _pitch(C)
+    sr, sc = s.stride(-2), s.stride(-1)
+    return v, ld, z, int(transposed), s, s.stride(0) if stack else 0, *((sc, sr) if rows_are_k else (sr, sc))
 
 
-def _operand(v: torch.Tensor, s: torch.Tensor, transposed: bool, along_k_is_row: bool):
-    """(values, row distance, matrix distance, transposed, scales and their distances: matrices, along M or N, along K)."""
-    Z, R, C = v.shape
-    ld = v.stride(1) if R > 1 else -(-C // 16) * 16
-    sz, sr, sc = s.stride()
-    mn, k = (sc, sr) if along_k_is_row else (sr, sc)
-    return (v, ld, v.stride(0), int(transposed), s, sz, mn, k)
-
-
-def _contract(mode: int, a, a_t: bool, b, b_t: bool, bias, out: torch.Tensor, out_ld: int, out_z: int, M: int, N: int, K: int,
-              L: int, a_rows: int = BLOCK):
-    """One call of the contraction.  ``a``, ``b``: (values [*, R, C], scales); ``a_t``: A is stored [K, M]; ``b_t``: B [N, K]."""
+def _contract(mode: int, a, b, bias, bias_z: int, out, out_ld: int, out_z: int, M: int, N: int, K: int, L: int,
+              a_rows: int = BLOCK):
+    """One call of the contraction.  ``a``, ``b``: as ``_operand`` describes them."""
     status = _status_word()
     parts = lib().query("clt_fp8_matmul_parts", mode, M, N, K, L, 0)
     ws = torch.empty(parts * M * N, dtype=torch.float32, device=out.device) if parts else None
-    lib().call("clt_fp8_matmul", mode, *_operand(*a, a_t, a_t), a_rows, *_operand(*b, b_t, not b_t), bias,
-               bias.stride(0) if bias is not None else 0, out, DTYPE_CODE[out.dtype], out_ld, out_z, ws, parts * M * N, M, N, K, L,
-               status, stream_ptr())
+    lib().call("clt_fp8_matmul", mode, *a, a_rows, *b, bias, bias_z, out, DTYPE_CODE[out.dtype], out_ld, out_z, ws, parts * M * N,
+               M, N, K, L, status, stream_ptr())
+
+
+def _matmul(a, b, bias, out_dtype):
+    va, vb = a.values, b.values
+    M, K = va.shape[-2:] if not a.transposed else (va.shape[-1], va.shape[-2])
+    N = vb.shape[-2] if b.transposed else vb.shape[-1]
+    Z = va.shape[0] if va.dim() == 3 else 1
+    out = torch.empty(*va.shape[:-2], M, N, dtype=out_dtype, device=va.device)
+    if out.numel() == 0:
+        return out
+    bias_z = 0
+    if bias is not None:
+        bias = bias.detach()
+        if bias.dtype != torch.float32 or bias.stride(-1) != 1:
+            bias = bias.float().contiguous()
+        bias_z = bias.stride(0) if bias.dim() == 2 else 0
+    if K == 0:
+        return out.zero_() if bias is None else out.copy_(bias.unsqueeze(-2).expand(out.shape) if bias.dim() == va.dim() - 1
+                                                           else bias.expand(out.shape))
+    _contract(_BATCHED, _operand(va, a.scales, a.transposed, a.transposed), _operand(vb, b.scales, not b.transposed, b.transposed),
+              bias, bias_z, out, N, M * N, M, N, K, Z, a.block_rows)
+    return out
 
 
 def matmul(a: BlockTensor, b: BlockTensor, bias: Optional[torch.Tensor] = None,
@@ -237,75 +266,109 @@ def matmul(a: BlockTensor, b: BlockTensor, bias: Optional[torch.Tensor] = None,
     rounded once to ``out_dtype``.  ``a`` has blocks of 1 x 128 or 128 x 128 (with 1 x 128 only untransposed: its blocks have to
     lie along the contraction), ``b`` blocks of 128 x 128; either may be a transposed view (``.mT``).  The products of the
     operands' scales have to be finite.  Values whose rows do not start on 16 bytes are copied first."""
-    for name, t in (("a", a), ("b", b)):
-        if not isinstance(t, BlockTensor):
-            raise TypeError(f"{name} must be a BlockTensor, got {type(t).__name__}")
-    _need(a.values.dim() == b.values.dim(), f"a {tuple(a.shape)} and b {tuple(b.shape)} must both be matrices or both stacks")
-    _need(a.device == b.device, f"a is on {a.device}, b on {b.device}")
-    _need(a.shape[-1] == b.shape[-2] and a.shape[:-2] == b.shape[:-2], f"a {tuple(a.shape)} does not match b {tuple(b.shape)}")
-    _need(b.block_rows == BLOCK, "b needs blocks of 128 x 128")
-    _need(a.block_rows == BLOCK or not a.transposed, "a transposed operand needs blocks of 128 x 128")
-    _need(out_dtype in DTYPE_CODE, f"the result is fp32, fp16 or bf16, not {out_dtype}")
-    (va, sa), (vb, sb) = a._stack(), b._stack()
-    Z, M, K, N = va.shape[0], a.shape[-2], a.shape[-1], b.shape[-1]
+    if not isinstance(a, BlockTensor) or not isinstance(b, BlockTensor):
+        raise TypeError(f"a and b must be BlockTensors, got {type(a).__name__} and {type(b).__name__}")
+    sa, sb = a.shape, b.shape
+    if len(sa) != len(sb):
+        raise ValueError(f"a {tuple(sa)} and b {tuple(sb)} must both be matrices or both stacks")
+    if a.device != b.device:
+        raise ValueError(f"a is on {a.device}, b on {b.device}")
+    if sa[-1] != sb[-2] or (len(sa) == 3 and sa[0] != sb[0]):
+        raise ValueError(f"a {tuple(sa)} does not match b {tuple(sb)}")
+    if b.block_rows != BLOCK:
+        raise ValueError("b needs blocks of 128 x 128")
+    if a.block_rows != BLOCK and a.transposed:
+        raise ValueError("a transposed operand needs blocks of 128 x 128")
+    if out_dtype not in DTYPE_CODE:
+        raise ValueError(f"the result is fp32, fp16 or bf16, not {out_dtype}")
     if bias is not None:
         _check("bias", bias, DTYPE_CODE, a.device)
-        _need(tuple(bias.shape) in ((N,), (Z, N)), f"bias {tuple(bias.shape)} does not match {(Z, N)}")
-        bias = bias.detach().float().expand(Z, N)
-        if bias.stride(1) != 1 and N > 1:
-            bias = bias.contiguous()
-    with _On(a.device):
-        out = torch.empty(*a.shape[:-1], N, dtype=out_dtype, device=a.device)
-        if out.numel() == 0:
-            return out
-        if K == 0:
-            return out.zero_() if bias is None else out.copy_(bias.unsqueeze(1).expand(Z, M, N).view(out.shape))
-        _contract(_BATCHED, (_aligned(va), sa), a.transposed, (_aligned(vb), sb), b.transposed, bias, out, N, M * N, M, N, K, Z,
-                  a.block_rows)
-    return out
+        if bias.shape != sb[-1:] and (len(sb) != 3 or bias.shape != (sb[0], sb[2])):
+            raise ValueError(f"bias {tuple(bias.shape)} does not match b {tuple(sb)}")
+    return _on(a.device, _matmul, a, b, bias, out_dtype)
 
 
 # ---- differentiable passes ------------------------------------------------------------------------------------------------------
-def _bias32(b):
-    return None if b is None else b.detach().float().contiguous()
+class _Copy:
+    """Where the 8-bit copy [Z, R, C] of a pass's operand is: one buffer, its values first, then its scales."""
+
+    __slots__ = ("buf", "Z", "R", "C", "at")
+
+    def __init__(self, Z, R, C, device=None, buf=None):
+        self.Z, self.R, self.C = Z, R, C
+        self.at = (Z * R * _pitch(C) + 3) & ~3              # bytes before the scales
+        self.buf = buf if buf is not None else \
+            torch.empty(self.at + 4 * Z * _blocks(R) * _blocks(C), dtype=torch.uint8, device=device)
+
+    def fill(self, x, x_ld, x_z, first=0, count=None, sums=None):
+        """Matrices first .. first + count from x."""
+        count = self.Z if count is None else count
+        p = self.buf.data_ptr()
+        _quantize(x, x_ld, x_z, count, self.R, self.C, BLOCK, p + first * self.R * _pitch(self.C),
+                  p + self.at + 4 * first * _blocks(self.R) * _blocks(self.C), sums)
+        return self
+
+    def operand(self, rows_are_k: bool, transposed: bool):
+        p, ld, rb, cb = self.buf.data_ptr(), _pitch(self.C), _blocks(self.R), _blocks(self.C)
+        return p, ld, self.R * ld, int(transposed), p + self.at, rb * cb, *((1, cb) if rows_are_k else (cb, 1))
+
+
+def _rows_first(x):
+    """x [B, L, C] with unit distance inside a row: (x, distance of rows, distance of layers)."""
+    if x.stride(2) != 1 and x.shape[2] > 1:
+        x = x.contiguous()
+    return x, x.stride(0), x.stride(1)
+
+
+def _project_forward(x, W, b, keep_x, keep_w):
+    B, L, D = x.shape
+    F = W.shape[2]
+    y = torch.empty(B, L, F, dtype=x.dtype, device=x.device)
+    xc = _Copy(L, B, D, x.device).fill(*_rows_first(x))
+    if W.stride(2) != 1:
+        W = W.contiguous()
+    wc = _Copy(L, D, F, x.device).fill(W, W.stride(1), W.stride(0))
+    if B:
+        b = None if b is None else b.detach().float().contiguous()
+        _contract(_BATCHED, xc.operand(False, False), wc.operand(True, False), b, F, y, L * F, F, B, F, D, L)
+    return y, xc.buf if keep_x else None, wc.buf if keep_w else None
+
+
+def _project_backward(g, x_buf, w_buf, dims, types, need):
+    B, L, D, F = dims
+    dev = g.device
+    dx = dW = None
+    db = torch.empty(L, F, dtype=torch.float32, device=dev) if need[2] else None
+    gc = _Copy(L, B, F, dev).fill(*_rows_first(g), sums=db)
+    if need[0]:
+        dx = torch.empty(B, L, D, dtype=types[0], device=dev)
+        if B:
+            _contract(_BATCHED, gc.operand(False, False), _Copy(L, D, F, buf=w_buf).operand(False, True), None, 0, dx, L * D, D,
+                      B, D, F, L)
+    if need[1]:
+        dW = torch.empty(L, D, F, dtype=types[1], device=dev)
+        if B:
+            _contract(_BATCHED, _Copy(L, B, D, buf=x_buf).operand(True, True), gc.operand(True, False), None, 0, dW, F, D * F,
+                      D, F, B, L)
+        else:
+            dW.zero_()
+    return dx, dW, db if db is None or types[2] == torch.float32 else db.to(types[2])
 
 
 class _Project(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b):
-        B, L, D = x.shape
-        F = W.shape[2]
-        ctx.dims, ctx.types = (B, L, D, F), (x.dtype, W.dtype, None if b is None else b.dtype)
-        with _On(x.device):
-            y = torch.empty(B, L, F, dtype=x.dtype, device=x.device)
-            xv, xs, _ = _quantize(x.transpose(0, 1), BLOCK)
-            wv, ws, _ = _quantize(W, BLOCK)
-            if B:
-                _contract(_BATCHED, (xv, xs), False, (wv, ws), False, _bias32(b), y, L * F, F, B, F, D, L)
         need_x, need_w = ctx.needs_input_grad[:2]
-        ctx.save_for_backward(*((xv, xs) if need_w else (None, None)), *((wv, ws) if need_x else (None, None)))
+        y, x_buf, w_buf = _on(x.device, _project_forward, x, W, b, need_w, need_x)
+        ctx.dims = (*x.shape, W.shape[2])
+        ctx.types = x.dtype, W.dtype, None if b is None else b.dtype
+        ctx.save_for_backward(x_buf, w_buf)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        xv, xs, wv, ws = ctx.saved_tensors
-        B, L, D, F = ctx.dims
-        dx = dW = db = None
-        need_x, need_w, need_b = ctx.needs_input_grad
-        with _On(g.device):
-            gv, gs, db = _quantize(g.transpose(0, 1), BLOCK, sums=need_b)
-            if need_x:
-                dx = torch.empty(B, L, D, dtype=ctx.types[0], device=g.device)
-                if B:
-                    _contract(_BATCHED, (gv, gs), False, (wv, ws), True, None, dx, L * D, D, B, D, F, L)
-            if need_w:
-                dW = torch.empty(L, D, F, dtype=ctx.types[1], device=g.device)
-                if B:
-                    _contract(_BATCHED, (xv, xs), True, (gv, gs), False, None, dW, F, D * F, D, F, B, L)
-                else:
-                    dW.zero_()
-        return dx, dW, db.to(ctx.types[2]) if need_b else None
+        return _on(g.device, _project_backward, g, *ctx.saved_tensors, ctx.dims, ctx.types, ctx.needs_input_grad)
 
 
 def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -315,66 +378,81 @@ def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) 
     the incoming gradient; one call keeps ``B L D + L D F`` bytes."""
     _check("x", x, DTYPE_CODE)
     _check("W", W, DTYPE_CODE, x.device)
-    _need(W.dim() in (2, 3), f"expected W [D, F] or [L, D, F], got {tuple(W.shape)}")
-    one = W.dim() == 2
-    inner = tuple(W.shape[:2]) if not one else (W.shape[0],)
-    _need(x.dim() > len(inner) - 1 and tuple(x.shape[x.dim() - len(inner):]) == inner, f"x {tuple(x.shape)} does not match W {tuple(W.shape)}")
-    _need(W.numel() > 0, f"empty W {tuple(W.shape)}")
+    ws, xs = W.shape, x.shape
+    one = len(ws) == 2
+    if len(ws) not in (2, 3) or W.numel() == 0:
+        raise ValueError(f"expected W [D, F] or [L, D, F], not empty, got {tuple(ws)}")
+    inner = 1 if one else 2
+    if len(xs) < inner or xs[len(xs) - inner:] != ws[:inner]:
+        raise ValueError(f"x {tuple(xs)} does not match W {tuple(ws)}")
     if b is not None:
         _check("b", b, DTYPE_CODE, x.device)
-        _need(tuple(b.shape) == (W.shape[-1],) if one else tuple(b.shape) == (W.shape[0], W.shape[2]),
-              f"b {tuple(b.shape)} does not match W {tuple(W.shape)}")
-    lead = x.shape[:x.dim() - len(inner)]
+        if b.shape != (ws[-1:] if one else (ws[0], ws[2])):
+            raise ValueError(f"b {tuple(b.shape)} does not match W {tuple(ws)}")
+    if not one and len(xs) == 3:
+        return _Project.apply(x, W, b)
+    lead = xs[:len(xs) - inner]
     if one:
         W, b = W.unsqueeze(0), None if b is None else b.unsqueeze(0)
-    y = _Project.apply(x.reshape(lead.numel(), *W.shape[:2]), W, b)
-    return y.view(*lead, *((W.shape[2],) if one else (W.shape[0], W.shape[2])))
+    return _Project.apply(x.reshape(lead.numel(), *W.shape[:2]), W, b).view(*lead, *(ws[1:] if one else (ws[0], ws[2])))
+
+
+def _pairs(t: int) -> int:
+    return t * (t + 1) // 2
+
+
+def _decode_forward(f, b, blocks, keep_f, keep_w):
+    B, L, F = f.shape
+    D = blocks[0].shape[2]
+    y = torch.empty(B, L, D, dtype=f.dtype, device=f.device)
+    fc = _Copy(L, B, F, f.device).fill(*_rows_first(f))
+    wc = _Copy(_pairs(L), F, D, f.device)
+    for t, w in enumerate(blocks):
+        if w.stride(2) != 1:
+            w = w.contiguous()
+        wc.fill(w, w.stride(1), w.stride(0), first=_pairs(t), count=t + 1)
+    if B:
+        b = None if b is None else b.detach().float().contiguous()
+        _contract(_DEC_FWD, fc.operand(False, False), wc.operand(True, False), b, D, y, L * D, D, B, D, F, L)
+    return y, fc.buf if keep_f else None, wc.buf if keep_w else None
+
+
+def _decode_backward(g, f_buf, w_buf, dims, types, need):
+    B, L, F, D = dims
+    dev = g.device
+    df, dW = None, [None] * L
+    db = torch.empty(L, D, dtype=torch.float32, device=dev) if need[1] else None
+    gc = _Copy(L, B, D, dev).fill(*_rows_first(g), sums=db)
+    if need[0]:
+        df = torch.empty(B, L, F, dtype=types[0], device=dev)
+        if B:
+            _contract(_DEC_DFEAT, gc.operand(False, False), _Copy(_pairs(L), F, D, buf=w_buf).operand(False, True), None, 0, df,
+                      L * F, F, B, F, D, L)
+    if any(need[2:]):
+        flat = torch.empty(_pairs(L), F, D, dtype=torch.float32, device=dev)
+        if B:
+            _contract(_DEC_DW, _Copy(L, B, F, buf=f_buf).operand(True, True), gc.operand(True, False), None, 0, flat, D, F * D,
+                      F, D, B, L)
+        else:
+            flat.zero_()
+        dW = [flat[_pairs(t):_pairs(t + 1)].to(types[2][t]) if need[2 + t] else None for t in range(L)]
+    return (df, db if db is None or types[1] == torch.float32 else db.to(types[1]), *dW)
 
 
 class _CrosslayerDecode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, b, *blocks):
-        B, L, F = f.shape
-        D = blocks[0].shape[2]
-        P = L * (L + 1) // 2
-        ctx.dims, ctx.types = (B, L, F, D), (f.dtype, None if b is None else b.dtype, [w.dtype for w in blocks])
-        with _On(f.device):
-            y = torch.empty(B, L, D, dtype=f.dtype, device=f.device)
-            fv, fs, _ = _quantize(f.transpose(0, 1), BLOCK)
-            wv = _storage(P, F, D, device=f.device)
-            ws = torch.empty(P, _blocks(F), _blocks(D), dtype=torch.float32, device=f.device)
-            for t, w in enumerate(blocks):
-                at = slice(t * (t + 1) // 2, (t + 1) * (t + 2) // 2)
-                _quantize(w, BLOCK, into=(wv[at], ws[at]))
-            if B:
-                _contract(_DEC_FWD, (fv, fs), False, (wv, ws), False, _bias32(b), y, L * D, D, B, D, F, L)
-        need_f, need_w = ctx.needs_input_grad[0], any(ctx.needs_input_grad[2:])
-        ctx.save_for_backward(*((fv, fs) if need_w else (None, None)), *((wv, ws) if need_f else (None, None)))
+        need_w = any(ctx.needs_input_grad[2:])
+        y, f_buf, w_buf = _on(f.device, _decode_forward, f, b, blocks, need_w, ctx.needs_input_grad[0])
+        ctx.dims = (*f.shape, blocks[0].shape[2])
+        ctx.types = f.dtype, None if b is None else b.dtype, [w.dtype for w in blocks]
+        ctx.save_for_backward(f_buf, w_buf)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        fv, fs, wv, ws = ctx.saved_tensors
-        B, L, F, D = ctx.dims
-        df = db = None
-        need_f, need_b, *need_w = ctx.needs_input_grad
-        dW = [None] * L
-        with _On(g.device):
-            gv, gs, db = _quantize(g.transpose(0, 1), BLOCK, sums=need_b)
-            if need_f:
-                df = torch.empty(B, L, F, dtype=ctx.types[0], device=g.device)
-                if B:
-                    _contract(_DEC_DFEAT, (gv, gs), False, (wv, ws), True, None, df, L * F, F, B, F, D, L)
-            if any(need_w):
-                P = L * (L + 1) // 2
-                flat = torch.empty(P, F, D, dtype=torch.float32, device=g.device)
-                if B:
-                    _contract(_DEC_DW, (fv, fs), True, (gv, gs), False, None, flat, D, F * D, F, D, B, L)
-                else:
-                    flat.zero_()
-                dW = [flat[t * (t + 1) // 2:(t + 1) * (t + 2) // 2].to(ctx.types[2][t]) if need_w[t] else None for t in range(L)]
-        return (df, db.to(ctx.types[1]) if need_b else None, *dW)
+        return _on(g.device, _decode_backward, g, *ctx.saved_tensors, ctx.dims, ctx.types, ctx.needs_input_grad)
 
 
 def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -382,59 +460,82 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
     ``b[t]``), ``blocks[t]`` being ``[t + 1, F, D]``, as ``CrosslayerDecoder.forward``.  Types, rounding and what is kept for backward as
     in ``project``: ``B L F + P F D`` bytes for the P blocks of the decoder."""
     _check("features", features, DTYPE_CODE)
-    _need(features.dim() >= 2, f"expected features [..., L, F], got {tuple(features.shape)}")
-    L, F = features.shape[-2:]
-    blocks = list(blocks)
-    _need(L > 0 and len(blocks) == L, f"{len(blocks)} decoder blocks for {L} layers")
+    shape, blocks = features.shape, list(blocks)
+    if len(shape) < 2 or shape[-2] == 0 or len(blocks) != shape[-2]:
+        raise ValueError(f"{len(blocks)} decoder blocks do not match features {tuple(shape)}")
+    L, F = shape[-2:]
     for t, w in enumerate(blocks):
         _check(f"blocks[{t}]", w, DTYPE_CODE, features.device)
-        _need(w.dim() == 3 and w.shape[:2] == (t + 1, F) and w.shape[2] == blocks[0].shape[2],
-              f"blocks[{t}] {tuple(w.shape)} does not match {(t + 1, F, blocks[0].shape[-1])}")
+        if w.shape != (t + 1, F, blocks[0].shape[-1]) or w.numel() == 0:
+            raise ValueError(f"blocks[{t}] {tuple(w.shape)} does not match {(t + 1, F, blocks[0].shape[-1])}")
     D = blocks[0].shape[2]
-    _need(F > 0 and D > 0, f"empty decoder blocks {tuple(blocks[0].shape)}")
     if b is not None:
         _check("b", b, DTYPE_CODE, features.device)
-        _need(tuple(b.shape) == (L, D), f"b {tuple(b.shape)} does not match {(L, D)}")
-    lead = features.shape[:-2]
+        if b.shape != (L, D):
+            raise ValueError(f"b {tuple(b.shape)} does not match {(L, D)}")
+    if len(shape) == 3:
+        return _CrosslayerDecode.apply(features, b, *blocks)
+    lead = shape[:-2]
     return _CrosslayerDecode.apply(features.reshape(lead.numel(), L, F), b, *blocks).view(*lead, L, D)
+
+
+def _jump_relu_forward(x, theta, bw, bw_value):
+    R, C = x.shape
+    if x.stride(1) != 1 and C > 1:
+        x = x.contiguous()
+    y = torch.empty(R, C, dtype=x.dtype, device=x.device)
+    bits = torch.empty(R, (C + 7) // 8, dtype=torch.int16, device=x.device)
+    if R * C:
+        lib().call("clt_jump_relu_fwd", x, x.stride(0), theta, bw, bw_value, y, bits, DTYPE_CODE[x.dtype], R, C, stream_ptr())
+    return y, bits
+
+
+def _jump_relu_backward(g, bits, theta, bw, bw_value):
+    R, C = g.shape
+    if g.stride(1) != 1 and C > 1:
+        g = g.contiguous()
+    dx = torch.empty(R, C, dtype=g.dtype, device=g.device)
+    if theta is None:
+        dtheta, ws, n = None, None, 0
+    else:
+        dtheta = torch.empty(C, dtype=torch.float32, device=g.device)
+        n = lib().query("clt_jump_relu_chunks", R, C) * C
+        ws = torch.empty(n, dtype=torch.float32, device=g.device)
+    if R * C:
+        lib().call("clt_jump_relu_bwd", g, g.stride(0), bits, theta, bw, bw_value, dx, dtheta, ws, n, DTYPE_CODE[g.dtype], R, C,
+                   stream_ptr())
+    elif dtheta is not None:
+        dtheta.zero_()
+    return dx, dtheta
 
 
 class _JumpReLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, theta, bandwidth):
-        R, C = x.shape
-        on_device = isinstance(bandwidth, torch.Tensor)
-        ctx.bandwidth = 0.0 if on_device else float(bandwidth)
-        with _On(x.device):
-            if x.stride(1) != 1 and C > 1:
-                x = x.contiguous()
-            y = torch.empty(R, C, dtype=x.dtype, device=x.device)
-            bits = torch.empty(R, -(-C // 8), dtype=torch.int16, device=x.device)
-            th = None if theta is None else theta.detach().float().contiguous()
-            bw = bandwidth.detach().float() if on_device else None
-            if y.numel():
-                lib().call("clt_jump_relu_fwd", x, x.stride(0), th, bw, ctx.bandwidth, y, bits, DTYPE_CODE[x.dtype], R, C, stream_ptr())
-        ctx.theta_type = None if theta is None else theta.dtype
-        ctx.save_for_backward(bits, th, bw)
+        th, bw, value = theta, None, 0.0
+        if theta is not None:
+            if th.dtype != torch.float32 or not th.is_contiguous():
+                th = th.float().contiguous()
+            if isinstance(bandwidth, torch.Tensor):
+                bw = bandwidth if bandwidth.dtype == torch.float32 else bandwidth.float()
+            else:
+                value = float(bandwidth)
+        y, bits = _on(x.device, _jump_relu_forward, x, th, bw, value)
+        ctx.value = value
+        ctx.save_for_backward(bits, theta, bw)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        bits, th, bw = ctx.saved_tensors
-        R, C = g.shape
-        if g.stride(1) != 1 and C > 1:
-            g = g.contiguous()
-        dx = torch.empty(R, C, dtype=g.dtype, device=g.device)
-        dth = None if th is None else torch.zeros(C, dtype=torch.float32, device=g.device) if R == 0 else \
-            torch.empty(C, dtype=torch.float32, device=g.device)
-        with _On(g.device):
-            if dx.numel():
-                n = lib().query("clt_jump_relu_chunks", R, C) * C if th is not None else 0
-                ws = torch.empty(n, dtype=torch.float32, device=g.device) if n else None
-                lib().call("clt_jump_relu_bwd", g, g.stride(0), bits, th, bw, ctx.bandwidth, dx, dth, ws, n, DTYPE_CODE[g.dtype], R, C,
-                           stream_ptr())
-        return dx, None if dth is None else dth.to(ctx.theta_type), None
+        bits, theta, bw = ctx.saved_tensors
+        th = theta
+        if th is not None and (th.dtype != torch.float32 or not th.is_contiguous()):
+            th = th.float().contiguous()
+        dx, dtheta = _on(g.device, _jump_relu_backward, g, bits, th, bw, ctx.value)
+        if dtheta is not None and theta.dtype != torch.float32:
+            dtheta = dtheta.to(theta.dtype)
+        return dx, dtheta, None
 
 
 def jump_relu(x: torch.Tensor, theta: Optional[torch.Tensor] = None, bandwidth=1.0) -> torch.Tensor:
@@ -445,23 +546,22 @@ def jump_relu(x: torch.Tensor, theta: Optional[torch.Tensor] = None, bandwidth=1
     or one on ``x``'s device."""
     _check("x", x, DTYPE_CODE)
     shape = x.shape
-    _need(x.dim() >= 1, "x has no axis")
-    if theta is None:
-        C = shape[-1]
-        flat = None
-    else:
+    if len(shape) == 0:
+        raise ValueError("x has no axis")
+    C = shape[-1]
+    if theta is not None:
         _check("theta", theta, DTYPE_CODE, x.device)
-        inner = tuple(theta.shape)
-        while len(inner) > 1 and inner[0] == 1 and inner != tuple(shape[len(shape) - len(inner):]):
+        inner = theta.shape
+        while len(inner) > 1 and inner[0] == 1 and inner != shape[len(shape) - len(inner):]:
             inner = inner[1:]
-        _need(len(inner) >= 1 and len(inner) <= len(shape) and tuple(shape[len(shape) - len(inner):]) == inner,
-              f"theta {tuple(theta.shape)} does not match the last axes of x {tuple(shape)}")
-        C = theta.numel()
-        flat = theta.reshape(C)
+        if not 1 <= len(inner) <= len(shape) or inner != shape[len(shape) - len(inner):]:
+            raise ValueError(f"theta {tuple(theta.shape)} does not match the last axes of x {tuple(shape)}")
+        C = inner.numel()
         if isinstance(bandwidth, torch.Tensor):
             _check("bandwidth", bandwidth, DTYPE_CODE, x.device)
-            _need(bandwidth.numel() == 1, f"bandwidth has {bandwidth.numel()} elements")
-        else:
-            _need(float(bandwidth) > 0, f"bandwidth must be positive, got {bandwidth}")
-    rows = x.numel() // C if C else 0
-    return _JumpReLU.apply(x.reshape(rows, C), flat, bandwidth).view(shape)
+            if bandwidth.numel() != 1:
+                raise ValueError(f"bandwidth has {bandwidth.numel()} elements")
+        elif not float(bandwidth) > 0:
+            raise ValueError(f"bandwidth must be positive, got {bandwidth}")
+        theta = theta.reshape(C)
+    return _JumpReLU.apply(x.reshape(x.numel() // C if C else 0, C), theta, bandwidth).view(shape)
