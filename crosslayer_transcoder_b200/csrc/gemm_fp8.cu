@@ -9,17 +9,22 @@ namespace {
 
 inline long long up(long long a, long long b) { return (a + b - 1) / b; }
 
-// Pairs of CTAs where rounding the rows up to 256 adds at most an eighth and pairs fill half the chip.
+// Pairs of CTAs where rounding the rows up to 256 adds at most an eighth.  (They are about as fast a block as single CTAs, and
+// take a third less from L2.)
+bool pair_rows(int M) { return up(M, 256) * 16 <= up(M, 128) * 9; }
 bool use_pair(const GemmGeom& g, int sms) {
-  const long long n_tiles = up(g.N, f8::kBN), single = up(g.M, 128) * n_tiles * g.nz, pairs = up(g.M, 256) * n_tiles * g.nz;
-  return pairs >= sms / 2 && pairs * 16 <= single * 9;
+  return pair_rows(g.M) && up(g.M, 256) * up(g.N, f8::kBN) * g.nz >= sms / 2;
 }
 
-// Cuts the contraction into parts (gemm.cuh) where there are fewer output tiles than SMs, or chains so uneven that the longest
-// outlasts a fair share by half; sets g.kb_per_part and returns the number of parts, or 0 for whole chains.
+// Cuts the contraction into parts (gemm.cuh) where that is estimated faster; sets g.kb_per_part and returns the number of parts, or
+// 0 for whole chains.  Estimates, in us: 0.45 a block of 128 x 256 x 128 (a CTA's, or a pair's of 256 rows), 1.5 a tile for its
+// output and the next one's start; partial sums go to memory and back at 5 TB/s, behind a launch of 4.  Parts are tried that
+// fill 1 to 8 rounds of the chip: 257 x 120000 x 768 in 17 parts of 58 blocks, 153 tiles, took 47 us, in 16 of 59, one
+// round, KEEP2; whole chains KEEP3.
 int plan_parts(GemmGeom& g, int sms) {
   const int kb_per_seg = (int)up(g.Kseg, f8::kBK);
-  const long long tiles = up(g.M, 128) * up(g.N, f8::kBN);
+  const bool pair = pair_rows(g.M);
+  const long long tiles = up(g.M, pair ? 256 : 128) * up(g.N, f8::kBN), workers = pair ? sms / 2 : sms;
   long long total = 0, longest = 0;
   for (int z = 0; z < g.nz; ++z) {
     const long long n = (long long)seg_count(g, z) * kb_per_seg;
@@ -27,13 +32,35 @@ int plan_parts(GemmGeom& g, int sms) {
     longest = n > longest ? n : longest;
   }
   g.kb_per_part = 0;
-  if (longest < 8 || longest * sms * 2 <= total * tiles * 3) return 0;
-  const long long share = up(total * tiles, sms), part = share < 4 ? 4 : share;
-  g.kb_per_part = (int)part;
-  long long parts = 0;
+  if (longest < 8) return 0;
+  const double block = 0.45, tile = 1.5;
+  // equal chains run in rounds, unequal ones are dealt out longest first
+  const double whole = longest * g.nz == total
+                           ? up(tiles * g.nz, workers) * (longest * block + tile)
+                           : fmax(longest * block + tile, (total * block + g.nz * tile) * tiles / workers);
+  double best = 0.95 * whole;
+  int best_part = 0;
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    const long long room = rounds * workers / tiles;  // parts that these rounds have room for
+    if (room <= g.nz) continue;
+    GemmGeom h = g;
+    long long parts = 0;
+    const long long least = up(total, room);
+    for (long long p = least < 4 ? 4 : least; p < longest; ++p) {  // (grows by the slabs' last, shorter parts: few steps)
+      h.kb_per_part = (int)p;
+      parts = 0;
+      for (int z = 0; z < g.nz; ++z) parts += part_count(h, z, kb_per_seg);
+      if (parts <= room) break;
+    }
+    if (parts == 0 || parts > room || parts > 65535) continue;
+    const double us = rounds * (h.kb_per_part * block + tile) + 4.0 + 8.0 * parts * g.M * g.N / 5e6;
+    if (us < best) best = us, best_part = h.kb_per_part;
+  }
+  if (best_part == 0) return 0;
+  g.kb_per_part = best_part;
+  int parts = 0;
   for (int z = 0; z < g.nz; ++z) parts += part_count(g, z, kb_per_seg);
-  if (parts <= g.nz || parts > 65535) return g.kb_per_part = 0;
-  return (int)parts;
+  return parts;
 }
 
 template <class T>
@@ -51,11 +78,11 @@ struct FromFloat<__nv_bfloat16> {
   __device__ static __nv_bfloat16 get(float v) { return __float2bfloat16_rn(v); }
 };
 
-// out[z, m, n] = bias[z, n] + the partial sums of z's parts, in their order.
-template <class T>
-__global__ void __launch_bounds__(256) fp8_sum_parts_kernel(const float* __restrict__ ws, f8::Out out, GemmGeom g, int kb_per_seg) {
+// out[z, m, n] = bias[z, n] + the partial sums of z's parts, in their order.  V consecutive n to a thread (N a multiple of V).
+template <class T, int V>
+__global__ void __launch_bounds__(128) fp8_sum_parts_kernel(const float* __restrict__ ws, f8::Out out, GemmGeom g, int kb_per_seg) {
   const int z = blockIdx.y;
-  const long long slab = (long long)g.M * g.N, i = blockIdx.x * 256ll + threadIdx.x;
+  const long long slab = (long long)g.M * g.N, i = (blockIdx.x * 128ll + threadIdx.x) * V;
   if (i >= slab) return;
   int first = 0;
   for (int u = 0; u < z; ++u) first += part_count(g, u, kb_per_seg);
@@ -63,10 +90,32 @@ __global__ void __launch_bounds__(256) fp8_sum_parts_kernel(const float* __restr
   const long long m = i / g.N;
   const int n = (int)(i - m * g.N);
   const float* p = ws + first * slab + i;
-  float acc = out.bias != nullptr ? __ldg(out.bias + z * out.bias_z + n) : 0.f;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = out.bias != nullptr ? __ldg(out.bias + z * out.bias_z + n + k) : 0.f;
 #pragma unroll 8
-  for (int j = 0; j < parts; ++j) acc += __ldcs(p + j * slab);
-  ((T*)out.p)[z * out.z + m * out.ld + n] = FromFloat<T>::get(acc);
+  for (int j = 0; j < parts; ++j) {
+    if constexpr (V == 4) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(p + j * slab));
+      acc[0] += v.x, acc[1] += v.y, acc[2] += v.z, acc[3] += v.w;
+    } else {
+      acc[0] += __ldcs(p + j * slab);
+    }
+  }
+  T* o = (T*)out.p + z * out.z + m * out.ld + n;
+#pragma unroll
+  for (int k = 0; k < V; ++k) o[k] = FromFloat<T>::get(acc[k]);
+}
+
+template <class T>
+int sum_parts(const float* ws, const f8::Out& out, const GemmGeom& g, int kb_per_seg, cudaStream_t st) {
+  const long long slab = (long long)g.M * g.N;
+  if (g.N % 4 == 0)
+    fp8_sum_parts_kernel<T, 4><<<dim3((unsigned)up(slab, 512), g.nz), 128, 0, st>>>(ws, out, g, kb_per_seg);
+  else
+    fp8_sum_parts_kernel<T, 1><<<dim3((unsigned)up(slab, 128), g.nz), 128, 0, st>>>(ws, out, g, kb_per_seg);
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
 }
 
 template <bool A_MN, bool B_MN, bool kPair, int kOut, bool kByRow>
@@ -175,17 +224,11 @@ int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_tra
       gp.nz = parts;
       const f8::Out po{ws, 0, N, slab, nullptr, 0, N % 4 == 0};
       if (int rc = dispatch(gp, ta, tb, fa, fb, po, status, sms, (cudaStream_t)stream)) return rc;
-      const dim3 grid((unsigned)up(slab, 256), g.nz);
       const int kps = (int)up(K, f8::kBK);
       gp.nz = g.nz;
-      if (out_dtype == 0)
-        fp8_sum_parts_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
-      else if (out_dtype == 1)
-        fp8_sum_parts_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
-      else
-        fp8_sum_parts_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(ws, fo, gp, kps);
-      CLT_CHECK_CUDA(cudaGetLastError());
-      return 0;
+      if (out_dtype == 0) return sum_parts<float>(ws, fo, gp, kps, (cudaStream_t)stream);
+      if (out_dtype == 1) return sum_parts<__half>(ws, fo, gp, kps, (cudaStream_t)stream);
+      return sum_parts<__nv_bfloat16>(ws, fo, gp, kps, (cudaStream_t)stream);
     }
   }
   return dispatch(g, ta, tb, fa, fb, fo, status, sms, (cudaStream_t)stream);
