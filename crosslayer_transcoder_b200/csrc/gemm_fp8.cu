@@ -178,7 +178,7 @@ int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, 
 }
 
 bool geom(GemmGeom& g, int mode, int M, int N, int K, int L) {
-  if (mode < 0 || mode > 3 || M <= 0 || N <= 0 || K <= 0 || L <= 0 || L > 4096) return false;
+  if (mode < 0 || mode > 3 || M <= 0 || N <= 0 || K <= 0 || L <= 0 || L > (mode == kBatched ? 65535 : 361)) return false;  // slabs: a grid's y
   g = GemmGeom{mode, M, N, K, L, mode == kDecDW ? L * (L + 1) / 2 : L};
   return true;
 }

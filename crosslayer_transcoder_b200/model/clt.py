@@ -9,7 +9,8 @@ The training step does not call these ``forward`` methods: it runs the fused CUD
 path of ``crosslayer_transcoder_b200.engine`` on the same parameters.  The per-layer
 ``forward_layer`` calls run on the same kernels when the stack belongs to a training
 module and the input is on the GPU; otherwise, and for folding and export, the eager
-definitions below apply.
+definitions below apply.  ``CrossLayerTranscoder.eight_bit`` runs the differentiable
+forward of the whole container on 8-bit operands (``crosslayer_transcoder_b200.fp8``).
 """
 from __future__ import annotations
 
@@ -20,6 +21,8 @@ import torch
 import yaml
 from torch import nn
 
+from .. import fp8
+from .jumprelu import JumpReLU, ReLU
 from .serializable_module import SerializableModule
 from .standardize import Standardizer
 
@@ -167,6 +170,11 @@ class CrosslayerDecoder(_Layered):
 
 
 class CrossLayerTranscoder(SerializableModule):
+    #: Run ``forward`` on 8-bit operands (CUDA only, with or without gradients): encoder and decoder multiply block-scaled e4m3
+    #: copies, which backward reads again, and the (Jump)ReLU keeps two bits an element, so that a pass keeps a byte per
+    #: input, weight and feature where the eager definitions keep four, and four more per pre-activation.
+    eight_bit = False
+
     def __init__(self, nonlinearity: SerializableModule, encoder: Encoder,
                  decoder: Union[Decoder, CrosslayerDecoder],
                  input_standardizer: Optional[Standardizer] = None,
@@ -190,11 +198,31 @@ class CrossLayerTranscoder(SerializableModule):
         (reference clt.py:403-425)."""
         if self.input_standardizer is not None:
             acts = self.input_standardizer(acts)
-        pre_actvs = self.encoder(acts)
-        features = self.nonlinearity(pre_actvs)
-        recons_norm = self.decoder(features)
+        if self.eight_bit:
+            pre_actvs, features, recons_norm = self._forward_eight_bit(acts)
+        else:
+            pre_actvs = self.encoder(acts)
+            features = self.nonlinearity(pre_actvs)
+            recons_norm = self.decoder(features)
         recons = self.output_standardizer(recons_norm) if self.output_standardizer is not None else recons_norm
         return pre_actvs, features, recons_norm, recons
+
+    def _forward_eight_bit(self, acts):
+        """The three products of ``forward`` through ``crosslayer_transcoder_b200.fp8``, results in the type of ``acts``.  Nonlinearities
+        other than (Jump)ReLU are the module's own."""
+        enc, dec, nl = self.encoder, self.decoder, self.nonlinearity
+        pre_actvs = fp8.project(acts, enc.W, enc.b)
+        if isinstance(nl, JumpReLU):
+            features = fp8.jump_relu(pre_actvs, nl.theta, nl.bandwidth)
+        elif isinstance(nl, (ReLU, nn.ReLU)):
+            features = fp8.jump_relu(pre_actvs)
+        else:
+            features = nl(pre_actvs)
+        if dec.crosslayer:
+            recons_norm = fp8.crosslayer_decode(features, dec.blocks(), dec.b)
+        else:
+            recons_norm = fp8.project(features, dec.W, dec.b)
+        return pre_actvs, features, recons_norm
 
     def _init_args(self):
         sub = lambda m: None if m is None else m.to_config()

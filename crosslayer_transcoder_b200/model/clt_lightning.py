@@ -96,8 +96,9 @@ class CrossLayerTranscoderModule(_Base):
     def forward(self, acts_norm):
         """``(pre_actvs, features, recons_norm, recons)`` (reference clt_lightning.py:121-129).  On CUDA
         tensors with gradients disabled (validation, metrics) the two contractions run on this library's
-        kernels (``StepEngine.infer``); otherwise this is the model's differentiable PyTorch forward."""
-        if acts_norm.is_cuda and not torch.is_grad_enabled():
+        kernels (``StepEngine.infer``); otherwise this is the model's differentiable forward: PyTorch, or with
+        ``model.eight_bit`` (then without gradients too) 8-bit operands on this library's kernels."""
+        if acts_norm.is_cuda and not torch.is_grad_enabled() and not getattr(self.model, "eight_bit", False):
             return self._engine.infer(acts_norm)
         return self.model(acts_norm)
 

@@ -1,0 +1,150 @@
+"""What the 8-bit operators refuse, their plans and their status word: nothing here launches a kernel."""
+import pytest
+import torch
+
+from crosslayer_transcoder_b200 import fp8
+from crosslayer_transcoder_b200._lib import CltError, lib
+from crosslayer_transcoder_b200.model import CrosslayerDecoder, CrossLayerTranscoder, Encoder, JumpReLU
+
+
+def _block(R=256, C=256, rows=128, Z=None):
+    lead = () if Z is None else (Z,)
+    return fp8.BlockTensor(torch.zeros(*lead, R, C).to(torch.float8_e4m3fn), torch.ones(*lead, -(-R // rows), -(-C // 128)), rows)
+
+
+@pytest.mark.parametrize("call, error", [
+    (lambda: fp8.quantize([1.0]), TypeError),
+    (lambda: fp8.quantize(torch.zeros(4, 4, dtype=torch.float64)), TypeError),
+    (lambda: fp8.quantize(torch.zeros(4)), ValueError),
+    (lambda: fp8.quantize(torch.zeros(1, 1, 4, 4)), ValueError),
+    (lambda: fp8.quantize(torch.zeros(4, 4), block_rows=64), ValueError),
+    (lambda: fp8.BlockTensor(torch.zeros(4, 4), torch.ones(1, 1)), TypeError),
+    (lambda: fp8.BlockTensor(torch.zeros(4, 4).to(torch.float8_e4m3fn), torch.ones(1, 2)), ValueError),
+    (lambda: fp8.BlockTensor(torch.zeros(4, 4).to(torch.float8_e4m3fn), torch.ones(4, 1)), ValueError),
+    (lambda: fp8.BlockTensor(torch.zeros(4, 4).to(torch.float8_e4m3fn), torch.ones(1, 1).double()), TypeError),
+    (lambda: fp8.BlockTensor(torch.zeros(4, 4).to(torch.float8_e4m3fn), torch.ones(1, 1), block_rows=2), ValueError),
+    (lambda: _block()[0], ValueError),
+    (lambda: _block(Z=2)[0:1], ValueError),
+    (lambda: _block().dequantize(torch.float64), ValueError),
+    (lambda: fp8.matmul(torch.zeros(4, 4), _block()), TypeError),
+    (lambda: fp8.matmul(_block(), _block(Z=1)), ValueError),
+    (lambda: fp8.matmul(_block(C=128), _block()), ValueError),
+    (lambda: fp8.matmul(_block(Z=2), _block(Z=3)), ValueError),
+    (lambda: fp8.matmul(_block(), _block(rows=1)), ValueError),
+    (lambda: fp8.matmul(_block(rows=1).mT, _block()), ValueError),
+    (lambda: fp8.matmul(_block(), _block(), out_dtype=torch.float64), ValueError),
+    (lambda: fp8.matmul(_block(), _block(), bias=torch.zeros(255)), ValueError),
+    (lambda: fp8.matmul(_block(), _block(), bias=torch.zeros(256, dtype=torch.int32)), TypeError),
+    (lambda: fp8.project(torch.zeros(2, 3, 4), torch.zeros(3, 5, 6)), ValueError),
+    (lambda: fp8.project(torch.zeros(2, 2, 4), torch.zeros(3, 4, 6)), ValueError),
+    (lambda: fp8.project(torch.zeros(4), torch.zeros(3, 4, 6)), ValueError),
+    (lambda: fp8.project(torch.zeros(2, 4), torch.zeros(4)), ValueError),
+    (lambda: fp8.project(torch.zeros(2, 0), torch.zeros(0, 3)), ValueError),
+    (lambda: fp8.project(torch.zeros(2, 4), torch.zeros(4, 6), torch.zeros(5)), ValueError),
+    (lambda: fp8.project(torch.zeros(2, 4).long(), torch.zeros(4, 6)), TypeError),
+    (lambda: fp8.crosslayer_decode(torch.zeros(5, 2, 4), [torch.zeros(1, 4, 3)]), ValueError),
+    (lambda: fp8.crosslayer_decode(torch.zeros(5, 2, 4), [torch.zeros(1, 4, 3), torch.zeros(1, 4, 3)]), ValueError),
+    (lambda: fp8.crosslayer_decode(torch.zeros(5, 2, 4), [torch.zeros(1, 4, 3), torch.zeros(2, 4, 2)]), ValueError),
+    (lambda: fp8.crosslayer_decode(torch.zeros(5, 1, 4), [torch.zeros(1, 4, 3)], torch.zeros(3)), ValueError),
+    (lambda: fp8.crosslayer_decode(torch.zeros(5, 0, 4), []), ValueError),
+    (lambda: fp8.jump_relu(torch.tensor(1.0)), ValueError),
+    (lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(3)), ValueError),
+    (lambda: fp8.jump_relu(torch.zeros(4), torch.zeros(2, 4)), ValueError),
+    (lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(4), bandwidth=0.0), ValueError),
+    (lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(4), bandwidth=float("nan")), ValueError),
+    (lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(4), bandwidth=torch.ones(2)), ValueError),
+])
+def test_refusals(call, error):
+    with pytest.raises(error):
+        call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: fp8.quantize(torch.zeros(4, 4)),
+    lambda: _block().dequantize(),
+    lambda: fp8.matmul(_block(), _block()),
+    lambda: fp8.project(torch.zeros(2, 4), torch.zeros(4, 6)),
+    lambda: fp8.crosslayer_decode(torch.zeros(5, 1, 4), [torch.zeros(1, 4, 3)]),
+    lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(4)),
+])
+def test_cpu_tensors_are_refused(call):
+    with pytest.raises(CltError, match="CUDA"):
+        call()
+
+
+def test_model_switch():
+    model = CrossLayerTranscoder(JumpReLU(0.03, 1.0, 2, 24), Encoder(8, 24, 2), CrosslayerDecoder(8, 24, 2))
+    x = torch.randn(3, 2, 8)
+    before = model(x)
+    assert "eight_bit" not in str(model.to_config()) and not model.eight_bit
+    model.eight_bit = True
+    with pytest.raises(CltError, match="CUDA"):
+        model(x)
+    model.eight_bit = False
+    assert all(torch.equal(a, b) for a, b in zip(before, model(x)))
+
+
+def test_views():
+    b = _block(100, 300, 1, Z=2)
+    assert b.shape == (2, 100, 300) and b.mT.shape == (2, 300, 100) and b[1].shape == (100, 300) and b.mT.mT.shape == b.shape
+    assert b[0].mT.shape == (300, 100) and "block_rows=1" in repr(b)
+
+
+@pytest.mark.parametrize("mode, M, N, K, L", [(0, 257, 768, 120000, 1), (0, 1, 768, 24576, 1), (0, 1, 1, 1, 1), (1, 257, 768, 10000, 12),
+                                              (2, 5, 10000, 768, 12), (3, 320, 2001, 7, 6), (0, 33, 200, 20000, 3), (1, 64, 64, 64, 361)])
+def test_parts_cover_the_contraction(mode, M, N, K, L):
+    """Parts are at least two to a slab where there are any, of four blocks or more each, and few enough for a grid."""
+    parts = lib().query("clt_fp8_matmul_parts", mode, M, N, K, L, 148)
+    slabs = L * (L + 1) // 2 if mode == 3 else L
+    chain = {0: 1, 1: L, 2: L, 3: 1}[mode] * -(-K // 128)
+    assert parts == 0 or (slabs < parts <= 65535 and parts <= slabs * -(-chain // 4))
+    assert lib().query("clt_fp8_matmul_parts", mode, M, N, 0, L, 148) == 0
+
+
+def test_status_word(monkeypatch):
+    """What a kernel reports reaches the next call, once."""
+    word = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(fp8, "_status", word)
+    monkeypatch.setattr(fp8, "_status_view", word.numpy())
+    assert fp8._status_word() is word
+    word[0] = 0x12
+    with pytest.raises(CltError, match="0x12.*gave up waiting for an accumulator"):
+        fp8._status_word()
+    assert fp8._status_word() is word
+
+
+def test_library_refuses():
+    """Arguments that the library itself checks, before any launch."""
+    call = lib().call
+    p = 4096                                            # an address; nothing is read
+    with pytest.raises(CltError, match="blocks of 2 rows"):
+        call("clt_fp8_quantize", p, 0, 128, 0, p, 128, p, None, 1, 1, 128, 2, None)
+    with pytest.raises(CltError, match="column sums"):
+        call("clt_fp8_quantize", p, 0, 128, 0, p, 128, p, p, 1, 1, 128, 1, None)
+    with pytest.raises(CltError, match="16-byte aligned"):
+        call("clt_fp8_quantize", p, 0, 100, 0, p, 100, p, None, 1, 1, 100, 1, None)
+    with pytest.raises(CltError, match="misaligned"):
+        call("clt_fp8_quantize", p + 2, 0, 128, 0, p, 128, p, None, 1, 1, 128, 1, None)
+    with pytest.raises(CltError, match="null"):
+        call("clt_fp8_dequantize", None, 128, 0, p, 1, 1, 1, 1, p, 0, 1, 1, 128, None)
+    with pytest.raises(CltError, match="output type"):
+        call("clt_fp8_dequantize", p, 128, 0, p, 1, 1, 1, 1, p, 3, 1, 1, 128, None)
+    args = [0, p, 128, 0, 0, p, 1, 1, 1, 128, p, 128, 0, 0, p, 1, 1, 1, None, 0, p, 0, 128, 0, None, 0, 128, 128, 128, 1, p, None]
+    for at, value, text in ((0, 4, "bad mode"), (28, 0, "bad mode"), (29, 0, "bad mode"), (9, 2, "blocks of 2"), (21, 3, "output type"),
+                            (22, 127, "distance"), (20, p + 2, "misaligned"), (30, None, "null")):
+        bad = list(args)
+        bad[at] = value
+        with pytest.raises(CltError, match=text):
+            call("clt_fp8_matmul", *bad)
+    bad = list(args)
+    bad[4], bad[9] = 1, 1
+    with pytest.raises(CltError, match="transposed operand needs 128"):
+        call("clt_fp8_matmul", *bad)
+    with pytest.raises(CltError, match="bandwidth"):
+        call("clt_jump_relu_fwd", p, 8, p, None, 0.0, p, p, 0, 1, 8, None)
+    with pytest.raises(CltError, match="null"):
+        call("clt_jump_relu_bwd", p, 8, p, p, None, 1.0, p, None, None, 0, 0, 1, 8, None)
+    with pytest.raises(CltError, match="scratch"):
+        call("clt_jump_relu_bwd", p, 8, p, p, None, 1.0, p, p, p, 3, 0, 1, 8, None)
+    with pytest.raises(CltError, match="bad dims"):
+        call("clt_sum_chunks", p, p, 0, 1, 8, None)
