@@ -166,14 +166,27 @@ struct Source {
   long long ld, z;  // elements
   int R, C;
   int vec;  // rows start on 16 bytes
+  __device__ __forceinline__ const void* matrix(int i, int e) const { return (const char*)x + i * z * e; }
+};
+// The decoder's blocks, tensors of their own: number t holds t + 1 matrices, one after another.
+constexpr int kMaxBlocks = 64;
+struct BlockList {
+  const void* block[kMaxBlocks];
+  long long ld, z;
+  int R, C, vec;
+  __device__ __forceinline__ const void* matrix(int i, int e) const {
+    int t = 0;
+    while (i > t) i -= ++t;
+    return (const char*)block[t] + i * z * e;
+  }
 };
 
 // One CTA per 128 x 128 block, 16 lanes x 8 values to a row, 8 rows to a thread: the block is read once, all of it at a time.
 // Magnitudes are compared as integers, two 16-bit ones at a time; where a block turns out to hold infinities or NaN they are
 // found again without those.
 // kSums: sums[z, block of rows, c] = the block's column sums (of what came in), for bias gradients.
-template <class T, bool kSums>
-__global__ void __launch_bounds__(256) quantize_tile_kernel(Source s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
+template <class T, bool kSums, class S>
+__global__ void __launch_bounds__(256) quantize_tile_kernel(const __grid_constant__ S s, uint8_t* __restrict__ q, int q_ld, float* __restrict__ scales,
                                                             float* __restrict__ sums, int row_blocks, int col_blocks) {
   using V = Vec8<T>;
   __shared__ uint32_t part[2][8];
@@ -181,7 +194,7 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(Source s, uint8_t* _
   const int g = threadIdx.x >> 4, c = cb * 128 + (threadIdx.x & 15) * 8;
   const int n = s.C - c;
   const bool vec = s.vec && n >= 8;
-  const T* x = (const T*)s.x + z * s.z + (long long)(rb * 128 + g) * s.ld + c;
+  const T* x = (const T*)s.matrix(z, sizeof(T)) + (long long)(rb * 128 + g) * s.ld + c;
   const int rows = s.R - rb * 128 - g;
   V v[8];
 #pragma unroll
@@ -474,10 +487,19 @@ int quantize(const Source& s, uint8_t* q, int q_ld, float* scales, float* sums, 
     CLT_CHECK_ARG(rb * cb < (1ll << 31) && Z <= 65535, "fp8_quantize: too many blocks");
     const dim3 grid((unsigned)(rb * cb), Z);
     if (sums != nullptr)
-      quantize_tile_kernel<T, true><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
+      quantize_tile_kernel<T, true, Source><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
     else
-      quantize_tile_kernel<T, false><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
+      quantize_tile_kernel<T, false, Source><<<grid, 256, 0, st>>>(s, q, q_ld, scales, sums, (int)rb, cb);
   }
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+template <class T>
+int quantize_list(const BlockList& s, uint8_t* q, int q_ld, float* scales, int Z, cudaStream_t st) {
+  const long long rb = up(s.R, 128), cb = up(s.C, 128);
+  CLT_CHECK_ARG(rb * cb < (1ll << 31), "fp8_quantize_blocks: too many blocks");
+  quantize_tile_kernel<T, false, BlockList><<<dim3((unsigned)(rb * cb), Z), 256, 0, st>>>(s, q, q_ld, scales, nullptr, (int)rb, (int)cb);
   CLT_CHECK_CUDA(cudaGetLastError());
   return 0;
 }
@@ -544,6 +566,30 @@ int clt_fp8_quantize(const void* x, int in_dtype, int64_t ld, int64_t z_stride, 
   if (in_dtype == 0) return quantize<float>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
   if (in_dtype == 1) return quantize<__half>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
   return quantize<__nv_bfloat16>(s, (uint8_t*)q, (int)q_ld, scales, column_sums, Z, block_rows, st);
+}
+
+int clt_fp8_quantize_blocks(const uint64_t* blocks, int n, int in_dtype, void* q, int64_t q_ld, float* scales, int R, int C,
+                            clt_stream_t stream) {
+  CLT_CHECK_ARG(blocks && q && scales, "fp8_quantize_blocks: null pointer");
+  CLT_CHECK_ARG(n > 0 && n <= kMaxBlocks && R > 0 && C > 0, "fp8_quantize_blocks: bad dims n=%d (at most %d) R=%d C=%d", n, kMaxBlocks,
+                R, C);
+  CLT_CHECK_ARG(in_dtype >= 0 && in_dtype <= 2, "fp8_quantize_blocks: input type %d", in_dtype);
+  CLT_CHECK_ARG(q_ld >= C && q_ld % 16 == 0 && q_ld < (1ll << 31) && aligned16(q),
+                "fp8_quantize_blocks: rows of the copy must be 16-byte aligned (distance %lld)", (long long)q_ld);
+  const int e = elem_size(in_dtype);
+  BlockList s{};
+  s.ld = C, s.z = (long long)R * C, s.R = R, s.C = C;
+  s.vec = (long long)C * e % 16 == 0;
+  for (int t = 0; t < n; ++t) {
+    s.block[t] = (const void*)(uintptr_t)blocks[t];
+    CLT_CHECK_ARG(s.block[t] != nullptr && blocks[t] % e == 0, "fp8_quantize_blocks: block %d is null or misaligned", t);
+    s.vec = s.vec && aligned16(s.block[t]);
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  const int Z = n * (n + 1) / 2;
+  if (in_dtype == 0) return quantize_list<float>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
+  if (in_dtype == 1) return quantize_list<__half>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
+  return quantize_list<__nv_bfloat16>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
 }
 
 int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,

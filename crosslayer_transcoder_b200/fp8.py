@@ -22,6 +22,7 @@ waits for the device first.
 """
 from __future__ import annotations
 
+from array import array
 from typing import Optional, Sequence
 
 import torch
@@ -407,10 +408,16 @@ def _decode_forward(f, b, blocks, keep_f, keep_w):
     y = torch.empty(B, L, D, dtype=f.dtype, device=f.device)
     fc = _Copy(L, B, F, f.device).fill(*_rows_first(f))
     wc = _Copy(_pairs(L), F, D, f.device)
-    for t, w in enumerate(blocks):
-        if w.stride(2) != 1:
-            w = w.contiguous()
-        wc.fill(w, w.stride(1), w.stride(0), first=_pairs(t), count=t + 1)
+    if L <= 64 and all(w.is_contiguous() and w.dtype == blocks[0].dtype for w in blocks):
+        at = array("Q", [w.data_ptr() for w in blocks])
+        p = wc.buf.data_ptr()
+        lib().call("clt_fp8_quantize_blocks", at.buffer_info()[0], L, DTYPE_CODE[blocks[0].dtype], p, _pitch(D), p + wc.at, F, D,
+                   stream_ptr())
+    else:
+        for t, w in enumerate(blocks):
+            if w.stride(2) != 1:
+                w = w.contiguous()
+            wc.fill(w, w.stride(1), w.stride(0), first=_pairs(t), count=t + 1)
     if B:
         b = None if b is None else b.detach().float().contiguous()
         _contract(_DEC_FWD, fc.operand(False, False), wc.operand(True, False), b, D, y, L * D, D, B, D, F, L)

@@ -490,6 +490,10 @@ int clt_cast_bf16(const float* src, void* dst, int64_t n, clt_stream_t stream);
 int clt_fp8_quantize(const void* x, int in_dtype, int64_t ld, int64_t z_stride, void* q, int64_t q_ld, float* scales,
                      float* column_sums, int Z, int R, int C, int block_rows, clt_stream_t stream);
 int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_stream_t stream);
+/* clt_fp8_quantize by blocks of 128 x 128 of the decoder's tensors, n <= 64 of them: blocks[t] (a host array of device addresses) is a
+ * contiguous [t + 1, R, C]; q and scales take their n (n + 1) / 2 matrices one after another. */
+int clt_fp8_quantize_blocks(const uint64_t* blocks, int n, int in_dtype, void* q, int64_t q_ld, float* scales, int R, int C,
+                            clt_stream_t stream);
 /* out [Z, R, C] (contiguous) = value * scale, rounded once.  s_z, s_r, s_c: distances of the scales between matrices, blocks
  * of rows and blocks of columns. */
 int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,

@@ -125,6 +125,10 @@ def test_library_refuses():
         call("clt_fp8_quantize", p, 0, 100, 0, p, 100, p, None, 1, 1, 100, 1, None)
     with pytest.raises(CltError, match="misaligned"):
         call("clt_fp8_quantize", p + 2, 0, 128, 0, p, 128, p, None, 1, 1, 128, 1, None)
+    one = torch.tensor([0], dtype=torch.int64)          # a host array with a null address
+    for n, text in ((0, "bad dims"), (65, "bad dims"), (1, "null")):
+        with pytest.raises(CltError, match=text):
+            call("clt_fp8_quantize_blocks", one, n, 0, p, 128, p, 4, 128, None)
     with pytest.raises(CltError, match="null"):
         call("clt_fp8_dequantize", None, 128, 0, p, 1, 1, 1, 1, p, 0, 1, 1, 128, None)
     with pytest.raises(CltError, match="output type"):

@@ -284,6 +284,28 @@ def test_crosslayer_decode(dims, dtype):
     fp8.check_status()
 
 
+def test_crosslayer_decode_block_forms():
+    """Blocks that are views, of mixed types or many give what contiguous fp32 ones do."""
+    L, F, D, B = 3, 72, 40, 30
+    f, b = torch.relu(_rand((B, L, F), 1)), _rand((L, D), 2)
+    wide = [_rand((t + 1, F, 2 * D), 3 + t).bfloat16().float() for t in range(L)]
+    views = [w[:, :, ::2] for w in wide]
+    want = fp8.crosslayer_decode(f, [v.contiguous() for v in views], b)
+    assert torch.equal(fp8.crosslayer_decode(f, views, b), want)
+    mixed = [v.contiguous().to(torch.bfloat16 if t == 1 else torch.float32).requires_grad_() for t, v in enumerate(views)]
+    y = fp8.crosslayer_decode(f, mixed, b)
+    assert torch.equal(y, want)
+    grads = torch.autograd.grad(y, mixed, torch.ones_like(y))
+    assert [g.dtype for g in grads] == [torch.float32, torch.bfloat16, torch.float32]
+    assert torch.equal(fp8.crosslayer_decode(f.view(5, 6, L, F), views, b), want.view(5, 6, L, D))
+    L = 66
+    f, ws = torch.relu(_rand((4, L, 8), 1)), [_rand((t + 1, 8, 16), t) for t in range(L)]
+    y = fp8.crosslayer_decode(f, ws)
+    fq, wq = ref.rounded(f.transpose(0, 1)), ref.rounded(ws[-1])
+    ref.check(y[:, -1], (fq @ wq).sum(0), (fq.abs() @ wq.abs()).sum(0), L * 8)
+    fp8.check_status()
+
+
 # ---- (Jump)ReLU ----------------------------------------------------------------------------------------------------------------
 def _jump_reference(x, theta, bw, g):
     x, g, th = x.double().cpu(), g.double().cpu(), theta.double().cpu()
