@@ -215,10 +215,7 @@ __device__ __forceinline__ uint4 pack_out(const float* v) {
                       pack16<__nv_bfloat16>(v[6], v[7]));
 }
 
-template <int kKeep>
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kKeep) : "memory");
-}
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
 // A warp's 32 rows x 128 columns of finished sums, to the output in the type kOut (as Out::dtype; one instantiation each: with all
 // three in one kernel the sums do not stay in registers).  Boxes of 32 rows x 128 B go through two buffers of shared memory
@@ -227,50 +224,53 @@ __device__ __forceinline__ void bulk_wait_read() {
 // (16-byte stores from registers through a small buffer, as in epi::store_rows32, took 2.4 us a tile, in which the tensor cores wait:
 // 12 x 4000 x 768 x 24576 1643 instead of 1318 us.)
 template <int kOut>
-__device__ __forceinline__ void store_warp(float (&acc)[128], const float* bias, uint8_t* buf, const CUtensorMap* map, const Out& o,
-                                           int z, int row0, int col0, int M, int N) {
+__device__ __forceinline__ void store_warp(const float (&acc)[128], uint8_t* buf, const CUtensorMap* map, const Out& o, int z, int row0,
+                                           int col0, int M, int N) {
   constexpr int kSize = kOut == 0 ? 4 : 2, kCols = 128 / kSize, kPer = 16 / kSize;
   const int lane = threadIdx.x & 31;
-  if (o.bias != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
-      acc[4 * i] += b.x, acc[4 * i + 1] += b.y, acc[4 * i + 2] += b.z, acc[4 * i + 3] += b.w;
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < 128 / kCols; ++c) {
-    uint8_t* box = buf + (c & 1) * 4096;
-    if (lane == 0) bulk_wait_read<1>();  // the copy before last, from this buffer, has been read
+  for (int c0 = 0; c0 < 128 / kCols; c0 += 2) {
+    if (lane == 0) bulk_wait_read();  // the buffers' last copies have been read
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = pack_out<kOut>(acc + c * kCols + i * kPer);
-    const int n = col0 + c * kCols;
+    for (int c = c0; c < c0 + 2; ++c) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(buf + (c & 1) * 4096 + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+            pack_out<kOut>(acc + c * kCols + i * kPer);
+    }
     if (o.tma) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
-        if (n < N)
-          asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                       "r"(tc::smem_u32(box)), "r"(n), "r"(row0), "r"(z)
-                       : "memory");
+#pragma unroll
+        for (int c = c0; c < c0 + 2; ++c) {
+          const int n = col0 + c * kCols;
+          if (n < N)
+            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+                         "r"(tc::smem_u32(buf + (c & 1) * 4096)), "r"(n), "r"(row0), "r"(z)
+                         : "memory");
+        }
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     } else {
       __syncwarp();
-      const int rows = min(32, M - row0), cols = min(kCols, N - n);
-      uint8_t* p = (uint8_t*)o.p + (z * o.z + (long long)row0 * o.ld + n) * kSize;
-#pragma unroll 1
-      for (int r = 0; r < rows; ++r) {
+      const int rows = min(32, M - row0);
 #pragma unroll
-        for (int k = lane; k < kCols; k += 32) {
-          if (k < cols) {
-            const uint8_t* v = box + r * 128 + (((k / kPer) ^ (r & 7)) << 4) + k % kPer * kSize;
-            if constexpr (kOut == 0)
-              *reinterpret_cast<uint32_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint32_t*>(v);
-            else
-              *reinterpret_cast<uint16_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint16_t*>(v);
+      for (int c = c0; c < c0 + 2; ++c) {
+        const int n = col0 + c * kCols, cols = min(kCols, N - n);
+        uint8_t* p = (uint8_t*)o.p + (z * o.z + (long long)row0 * o.ld + n) * kSize;
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r) {
+#pragma unroll
+          for (int k = lane; k < kCols; k += 32) {
+            if (k < cols) {
+              const uint8_t* v = buf + (c & 1) * 4096 + r * 128 + (((k / kPer) ^ (r & 7)) << 4) + k % kPer * kSize;
+              if constexpr (kOut == 0)
+                *reinterpret_cast<uint32_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint32_t*>(v);
+              else
+                *reinterpret_cast<uint16_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint16_t*>(v);
+            }
           }
         }
       }
@@ -503,7 +503,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           alive = __all_sync(0xffffffffu, ok);
           if (!alive) break;
           if (out.bias != nullptr && at == kb_lo) {
-            // with the tile's first window, once the tile kSlots before has been put out
+            // with the tile's first window; the tile kSlots before took its own before it gave a window back
 #pragma unroll
             for (int i = 0; i < kBN; i += 64)
               ring->bias[it % kSlots][i + t] = n0 + i + t < g.N ? __ldg(out.bias + zo * out.bias_z + n0 + i + t) : 0.f;
@@ -581,9 +581,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
       tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
       const int row0 = m0 + rank * kBM + quarter * 32, col0 = n0 + half * 128;
       const bool work = row0 < g.M && col0 < g.N;  // uniform over the warp: something of it is stored
-      float acc[128];
-#pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      float acc[128];  // begin with the bias, which comes with the tile's first window
       uint32_t r0[16], r1[16];
       // One read of tensor memory is in flight at any time, across the blocks: the next block's first is issued before this
       // block's last columns are added.
@@ -594,6 +592,19 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         const int slot = batch % kSlots;
         alive = wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutTmemFull);
         alive = __all_sync(0xffffffffu, alive);
+        if (left == kb_hi - kb_lo) {
+          if (out.bias != nullptr) {
+            const float* bias = ring->bias[it % kSlots] + half * 128;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
+              acc[4 * i] = b.x, acc[4 * i + 1] = b.y, acc[4 * i + 2] = b.z, acc[4 * i + 3] = b.w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+          }
+        }
         const float* ra = ring->a[slot] + (kByRow ? quarter * 32 + lane : 0);
         const float* rb = &ring->b[slot][0][half];
         const int groups = kByRow ? min(left, window) : __popc(ring->starts[slot]);
@@ -629,10 +640,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           }
           if (work) fma16(acc + 112, r1, s);
         }
-        if (left <= window && alive && work)  // before the slot is given back: the bias that it brought is read here
-          store_warp<kOut>(acc, ring->bias[it % kSlots] + half * 128, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->empty[slot]));
+        if (left <= window && alive && work) store_warp<kOut>(acc, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);
       }
     }
   }
