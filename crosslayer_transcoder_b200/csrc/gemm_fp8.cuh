@@ -66,6 +66,7 @@ struct alignas(16) ScaleRing {
   float a[kSlots][kByRow ? kWindow * 128 : kWindow];
   float b[kSlots][kWindow][2];
   float bias[kSlots][kBN];  // of tiles, which have a window each at least
+  int4 tile[kSlots];  // with a tile's first window: row, column, output slab, blocks (0: there are no more tiles)
   uint32_t starts[kSlots];
   uint64_t full[kSlots], empty[kSlots];
 };
@@ -502,6 +503,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
               wait(tc::smem_u32(&ring->empty[slot]), ((batch / kSlots) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty);
           alive = __all_sync(0xffffffffu, ok);
           if (!alive) break;
+          if (t == 0 && at == kb_lo) ring->tile[slot] = make_int4(m0 + rank * kBM, n0, zo, kb_hi - kb_lo);
           if (out.bias != nullptr && at == kb_lo) {
             // with the tile's first window; the tile kSlots before took its own before it gave a window back
 #pragma unroll
@@ -560,51 +562,57 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->full[slot]));
         }
       }
+      const int slot = batch % kSlots;
+      const bool ok =
+          alive && wait(tc::smem_u32(&ring->empty[slot]), ((batch / kSlots) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty);
+      if (__all_sync(0xffffffffu, ok)) {
+        if (t == 0) ring->tile[slot] = make_int4(0, 0, 0, 0);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->full[slot]));
+      }
     }
   } else {
     // ------------------------------ epilogue ----------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int ew = warp - kFirstEpiWarp;
     uint8_t* buf8 = out_smem + ew * kOutBytes;
+    const auto window_ready = [&](uint32_t batch) {
+      const bool ok = wait(tc::smem_u32(&ring->full[batch % kSlots]), (batch / kSlots) & 1, abort_flag, status, kTimeoutTmemFull);
+      return (bool)__all_sync(0xffffffffu, ok);
+    };
     const int quarter = warp & 3;  // tensor-memory lanes 32*quarter .. +31
     const int half = ew >> 2;      // which 128 columns of the tile
     const uint32_t tbase = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     uint32_t n = 0, batch = 0;
     bool alive = true;
+    // Which tile comes next arrives with its scales: the divisions that it takes are not made here, where the tensor cores would wait.
     for (int it = 0; alive; ++it) {
-      const long long tile_l = tc::tile_of_round(it, worker, workers);
-      if (tile_l >= total_tiles) break;
-      const int tile = (int)tile_l;
-      int z, kb_lo, kb_hi, zo;
-      work_item(g, tile / tiles_per_slab, kb_per_seg, z, kb_lo, kb_hi, zo);
-      int m0, n0;
-      tc::tile_origin(tile % tiles_per_slab, m_tiles, n_tiles, TL::kM, m0, n0);
-      const int row0 = m0 + rank * kBM + quarter * 32, col0 = n0 + half * 128;
+      if (!window_ready(batch)) break;
+      const int4 tile = ring->tile[batch % kSlots];
+      if (tile.w == 0) break;
+      const int row0 = tile.x + quarter * 32, col0 = tile.y + half * 128, zo = tile.z;
       const bool work = row0 < g.M && col0 < g.N;  // uniform over the warp: something of it is stored
-      float acc[128];  // begin with the bias, which comes with the tile's first window
       uint32_t r0[16], r1[16];
       // One read of tensor memory is in flight at any time, across the blocks: the next block's first is issued before this
       // block's last columns are added.
       alive = block_ready(bars, n, abort_flag, status);
       if (alive && work) tmem_ld16_issue(tbase + (n & 1) * kBN, r0);
-#pragma unroll 1
-      for (int left = kb_hi - kb_lo; left > 0 && alive; left -= window, ++batch) {
-        const int slot = batch % kSlots;
-        alive = wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutTmemFull);
-        alive = __all_sync(0xffffffffu, alive);
-        if (left == kb_hi - kb_lo) {
-          if (out.bias != nullptr) {
-            const float* bias = ring->bias[it % kSlots] + half * 128;
+      float acc[128];
+      if (out.bias != nullptr) {
+        const float* bias = ring->bias[it % kSlots] + half * 128;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
-              acc[4 * i] = b.x, acc[4 * i + 1] = b.y, acc[4 * i + 2] = b.z, acc[4 * i + 3] = b.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-          }
+        for (int i = 0; i < 32; ++i) {
+          const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
+          acc[4 * i] = b.x, acc[4 * i + 1] = b.y, acc[4 * i + 2] = b.z, acc[4 * i + 3] = b.w;
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      }
+#pragma unroll 1
+      for (int left = tile.w; left > 0 && alive; left -= window, ++batch) {
+        const int slot = batch % kSlots;
+        if (left < tile.w) alive = window_ready(batch);
         const float* ra = ring->a[slot] + (kByRow ? quarter * 32 + lane : 0);
         const float* rb = &ring->b[slot][0][half];
         const int groups = kByRow ? min(left, window) : __popc(ring->starts[slot]);
