@@ -357,19 +357,31 @@ def _project_backward(g, x_buf, w_buf, dims, types, need):
 
 
 class _Project(torch.autograd.Function):
+    """(Shapes are brought into the form [B, L, D] in here: views made outside would be nodes of the graph.)"""
+
     @staticmethod
     def forward(ctx, x, W, b):
         need_x, need_w = ctx.needs_input_grad[:2]
+        shapes = x.shape, W.shape, None if b is None else b.shape
+        if W.dim() == 2:
+            W = W.unsqueeze(0)
+        L, D, F = W.shape
+        out_shape = (*x.shape[:-1], F)
+        x = x.reshape(shapes[0].numel() // (L * D), L, D)
         y, x_buf, w_buf = _on(x.device, _project_forward, x, W, b, need_w, need_x)
-        ctx.dims = (*x.shape, W.shape[2])
+        ctx.dims, ctx.shapes = (x.shape[0], L, D, F), shapes
         ctx.types = x.dtype, W.dtype, None if b is None else b.dtype
         ctx.save_for_backward(x_buf, w_buf)
-        return y
+        return y.view(out_shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        return _on(g.device, _project_backward, g, *ctx.saved_tensors, ctx.dims, ctx.types, ctx.needs_input_grad)
+        B, L, D, F = ctx.dims
+        dx, dW, db = _on(g.device, _project_backward, g.reshape(B, L, F), *ctx.saved_tensors, ctx.dims, ctx.types,
+                         ctx.needs_input_grad)
+        xs, ws, bs = ctx.shapes
+        return (None if dx is None else dx.view(xs), None if dW is None else dW.view(ws), None if db is None else db.view(bs))
 
 
 def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -390,12 +402,7 @@ def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) 
         _check("b", b, DTYPE_CODE, x.device)
         if b.shape != (ws[-1:] if one else (ws[0], ws[2])):
             raise ValueError(f"b {tuple(b.shape)} does not match W {tuple(ws)}")
-    if not one and len(xs) == 3:
-        return _Project.apply(x, W, b)
-    lead = xs[:len(xs) - inner]
-    if one:
-        W, b = W.unsqueeze(0), None if b is None else b.unsqueeze(0)
-    return _Project.apply(x.reshape(lead.numel(), *W.shape[:2]), W, b).view(*lead, *(ws[1:] if one else (ws[0], ws[2])))
+    return _Project.apply(x, W, b)
 
 
 def _pairs(t: int) -> int:
@@ -450,16 +457,22 @@ class _CrosslayerDecode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, b, *blocks):
         need_w = any(ctx.needs_input_grad[2:])
+        ctx.shape = f.shape
+        L, F, D = *f.shape[-2:], blocks[0].shape[2]
+        f = f.reshape(f.numel() // (L * F), L, F)
         y, f_buf, w_buf = _on(f.device, _decode_forward, f, b, blocks, need_w, ctx.needs_input_grad[0])
-        ctx.dims = (*f.shape, blocks[0].shape[2])
+        ctx.dims = f.shape[0], L, F, D
         ctx.types = f.dtype, None if b is None else b.dtype, [w.dtype for w in blocks]
         ctx.save_for_backward(f_buf, w_buf)
-        return y
+        return y.view(*ctx.shape[:-1], D)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        return _on(g.device, _decode_backward, g, *ctx.saved_tensors, ctx.dims, ctx.types, ctx.needs_input_grad)
+        B, L, F, D = ctx.dims
+        df, *rest = _on(g.device, _decode_backward, g.reshape(B, L, D), *ctx.saved_tensors, ctx.dims, ctx.types,
+                        ctx.needs_input_grad)
+        return (None if df is None else df.view(ctx.shape), *rest)
 
 
 def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -480,32 +493,31 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
         _check("b", b, DTYPE_CODE, features.device)
         if b.shape != (L, D):
             raise ValueError(f"b {tuple(b.shape)} does not match {(L, D)}")
-    if len(shape) == 3:
-        return _CrosslayerDecode.apply(features, b, *blocks)
-    lead = shape[:-2]
-    return _CrosslayerDecode.apply(features.reshape(lead.numel(), L, F), b, *blocks).view(*lead, L, D)
+    return _CrosslayerDecode.apply(features, b, *blocks)
 
 
-def _jump_relu_forward(x, theta, bw, bw_value):
-    R, C = x.shape
+def _jump_relu_forward(x, C, theta, bw, bw_value):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    R = y.numel() // C if C else 0
+    x = x.reshape(R, C)
     if x.stride(1) != 1 and C > 1:
         x = x.contiguous()
-    y = torch.empty(R, C, dtype=x.dtype, device=x.device)
     bits = torch.empty(R, (C + 7) // 8, dtype=torch.int16, device=x.device)
     if R * C:
         lib().call("clt_jump_relu_fwd", x, x.stride(0), theta, bw, bw_value, y, bits, DTYPE_CODE[x.dtype], R, C, stream_ptr())
     return y, bits
 
 
-def _jump_relu_backward(g, bits, theta, bw, bw_value):
-    R, C = g.shape
+def _jump_relu_backward(g, C, bits, theta, bw, bw_value):
+    dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    R = dx.numel() // C if C else 0
+    g = g.reshape(R, C)
     if g.stride(1) != 1 and C > 1:
         g = g.contiguous()
-    dx = torch.empty(R, C, dtype=g.dtype, device=g.device)
     if theta is None:
         dtheta, ws, n = None, None, 0
     else:
-        dtheta = torch.empty(C, dtype=torch.float32, device=g.device)
+        dtheta = torch.empty(theta.shape, dtype=torch.float32, device=g.device)
         n = lib().query("clt_jump_relu_chunks", R, C) * C
         ws = torch.empty(n, dtype=torch.float32, device=g.device)
     if R * C:
@@ -518,7 +530,7 @@ def _jump_relu_backward(g, bits, theta, bw, bw_value):
 
 class _JumpReLU(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, theta, bandwidth):
+    def forward(ctx, x, theta, bandwidth, C):
         th, bw, value = theta, None, 0.0
         if theta is not None:
             if th.dtype != torch.float32 or not th.is_contiguous():
@@ -527,8 +539,8 @@ class _JumpReLU(torch.autograd.Function):
                 bw = bandwidth if bandwidth.dtype == torch.float32 else bandwidth.float()
             else:
                 value = float(bandwidth)
-        y, bits = _on(x.device, _jump_relu_forward, x, th, bw, value)
-        ctx.value = value
+        y, bits = _on(x.device, _jump_relu_forward, x, C, th, bw, value)
+        ctx.value, ctx.C = value, C
         ctx.save_for_backward(bits, theta, bw)
         return y
 
@@ -539,10 +551,10 @@ class _JumpReLU(torch.autograd.Function):
         th = theta
         if th is not None and (th.dtype != torch.float32 or not th.is_contiguous()):
             th = th.float().contiguous()
-        dx, dtheta = _on(g.device, _jump_relu_backward, g, bits, th, bw, ctx.value)
+        dx, dtheta = _on(g.device, _jump_relu_backward, g, ctx.C, bits, th, bw, ctx.value)
         if dtheta is not None and theta.dtype != torch.float32:
             dtheta = dtheta.to(theta.dtype)
-        return dx, dtheta, None
+        return dx, dtheta, None, None
 
 
 def jump_relu(x: torch.Tensor, theta: Optional[torch.Tensor] = None, bandwidth=1.0) -> torch.Tensor:
@@ -570,5 +582,4 @@ def jump_relu(x: torch.Tensor, theta: Optional[torch.Tensor] = None, bandwidth=1
                 raise ValueError(f"bandwidth has {bandwidth.numel()} elements")
         elif not float(bandwidth) > 0:
             raise ValueError(f"bandwidth must be positive, got {bandwidth}")
-        theta = theta.reshape(C)
-    return _JumpReLU.apply(x.reshape(x.numel() // C if C else 0, C), theta, bandwidth).view(shape)
+    return _JumpReLU.apply(x, theta, bandwidth, C)
