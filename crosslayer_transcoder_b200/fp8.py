@@ -78,20 +78,25 @@ def _check(name: str, t, dtypes, device=None):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
-_checked = set()
+_checked = set()        # devices that the library runs on
 
 
 def _on(device, fn, *args):
     """``fn(*args)`` with the operands' device as the current one."""
+    if device.index in _checked and device.type == "cuda" and torch._C._cuda_getDevice() == device.index:
+        return fn(*args)
     if device.type != "cuda":
         raise CltError(f"the 8-bit operators run on CUDA tensors only (no CPU fallback), got {device}")
-    if torch.cuda.is_initialized() and torch._C._cuda_getDevice() == device.index:
-        if device.index not in _checked:
-            lib().check_device()
-            _checked.add(device.index)
-        return fn(*args)
     with torch.cuda.device(device):
-        return _on(device, fn, *args)
+        lib().check_device()
+        _checked.add(device.index)
+        return fn(*args)
+
+
+def _first_order(backward):
+    """``once_differentiable``, whose wrapper is entered only where a graph of the gradient is asked for."""
+    once = once_differentiable(backward)
+    return lambda ctx, g: once(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
 
 
 def _pitch(C: int) -> int:
@@ -375,7 +380,7 @@ class _Project(torch.autograd.Function):
         return y.view(out_shape)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         B, L, D, F = ctx.dims
         dx, dW, db = _on(g.device, _project_backward, g.reshape(B, L, F), *ctx.saved_tensors, ctx.dims, ctx.types,
@@ -467,7 +472,7 @@ class _CrosslayerDecode(torch.autograd.Function):
         return y.view(*ctx.shape[:-1], D)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         B, L, F, D = ctx.dims
         df, *rest = _on(g.device, _decode_backward, g.reshape(B, L, D), *ctx.saved_tensors, ctx.dims, ctx.types,
@@ -499,21 +504,27 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
 def _jump_relu_forward(x, C, theta, bw, bw_value):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     R = y.numel() // C if C else 0
-    x = x.reshape(R, C)
-    if x.stride(1) != 1 and C > 1:
-        x = x.contiguous()
+    ld = C
+    if not x.is_contiguous():
+        x = x.reshape(R, C)
+        if x.stride(1) != 1 and C > 1:
+            x = x.contiguous()
+        ld = x.stride(0)
     bits = torch.empty(R, (C + 7) // 8, dtype=torch.int16, device=x.device)
     if R * C:
-        lib().call("clt_jump_relu_fwd", x, x.stride(0), theta, bw, bw_value, y, bits, DTYPE_CODE[x.dtype], R, C, stream_ptr())
+        lib().call("clt_jump_relu_fwd", x, ld, theta, bw, bw_value, y, bits, DTYPE_CODE[x.dtype], R, C, stream_ptr())
     return y, bits
 
 
 def _jump_relu_backward(g, C, bits, theta, bw, bw_value):
     dx = torch.empty(g.shape, dtype=g.dtype, device=g.device)
     R = dx.numel() // C if C else 0
-    g = g.reshape(R, C)
-    if g.stride(1) != 1 and C > 1:
-        g = g.contiguous()
+    ld = C
+    if not g.is_contiguous():
+        g = g.reshape(R, C)
+        if g.stride(1) != 1 and C > 1:
+            g = g.contiguous()
+        ld = g.stride(0)
     if theta is None:
         dtheta, ws, n = None, None, 0
     else:
@@ -521,7 +532,7 @@ def _jump_relu_backward(g, C, bits, theta, bw, bw_value):
         n = lib().query("clt_jump_relu_chunks", R, C) * C
         ws = torch.empty(n, dtype=torch.float32, device=g.device)
     if R * C:
-        lib().call("clt_jump_relu_bwd", g, g.stride(0), bits, theta, bw, bw_value, dx, dtheta, ws, n, DTYPE_CODE[g.dtype], R, C,
+        lib().call("clt_jump_relu_bwd", g, ld, bits, theta, bw, bw_value, dx, dtheta, ws, n, DTYPE_CODE[g.dtype], R, C,
                    stream_ptr())
     elif dtheta is not None:
         dtheta.zero_()
@@ -545,7 +556,7 @@ class _JumpReLU(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, g):
         bits, theta, bw = ctx.saved_tensors
         th = theta
