@@ -5,6 +5,9 @@
 // 1 where all are zero.  With a power of two the quotient x / s and the product q * s are exact, so that the only rounding is the
 // one to e4m3 (half a step: 2^-4 of the value), whichever way a copy was made, and a copy of a copy is the copy.  e4m3 has no
 // infinity: what is not finite becomes NaN, and does not count for the scale.
+//
+// All kernels here are bound by memory: 12 x 4000 x 10000 bf16 to 8 bits 231 us (6.2 TB/s), back 262 (5.5); a gradient with its column
+// sums, 12 x 4000 x 24576, 664 (5.3); (Jump)ReLU of that size 856 (5.9) and its backward 806 (6.2).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

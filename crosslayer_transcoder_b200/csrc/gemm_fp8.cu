@@ -20,7 +20,7 @@ bool use_pair(const GemmGeom& g, int sms) {
 // 0 for whole chains.  Estimates, in us: 0.45 a block of 128 x 256 x 128 (a CTA's, or a pair's of 256 rows), 1.5 a tile for its
 // output and the next one's start; partial sums go to memory and back at 5 TB/s, behind a launch of 4.  Parts are tried that
 // fill 1 to 8 rounds of the chip: 257 x 120000 x 768 in 17 parts of 58 blocks, 153 tiles, took 47 us, in 16 of 59, one
-// round, KEEP2; whole chains KEEP3.
+// round, 42; whole chains 500.
 int plan_parts(GemmGeom& g, int sms) {
   const int kb_per_seg = (int)up(g.Kseg, f8::kBK);
   const bool pair = pair_rows(g.M);

@@ -5,19 +5,27 @@
 //
 // A's scales belong to 1 x 128 or 128 x 128 blocks, B's to 128 x 128 blocks.  The inner sum runs in tensor memory (four
 // MMAs of 32); its 128 x 256 results then go through registers once, where they are scaled and added in fp32.  So a sum in
-// the tensor cores' own accumulator has 128 terms however long the contraction is, and any fp32 scales will do.
+// the tensor cores' own accumulator stays short however long the contraction is (error against 64 bits of a sum of 120000 products:
+// 1.4e-7), and any fp32 scales will do.
 //
-// Roles, barriers, operand layouts and pairs of CTAs are those of gemm_tc.cuh.  What differs:
-//   * A stage holds 128 of the contraction axis, one byte each: as many bytes as 64 bf16 values, twice the products.
+// Operand layouts, stages and pairs of CTAs are those of gemm_tc.cuh.  What differs:
+//   * A stage holds 128 of the contraction axis, one byte each: as many bytes as 64 bf16 values, twice the products.  Four stages
+//     (a pair; three for a CTA alone) are as fast as six and leave 64 KB for the output, which goes out by TMA.
 //   * The two accumulators of tensor memory alternate from block to block instead of from tile to tile: while the MMAs fill
 //     one, the eight epilogue warps read the other and add it to their 128 sums a thread (32 rows x 128 columns a warp).
-//     That is 32768 FMAs a block and SM, 256 cycles of the fp32 pipes beside 512 of the tensor cores; what it costs is the
-//     way from the MMAs to the epilogue and back, which two accumulators hide only in part
-//     (12 x 4000 x 24576 x 768: 924 us, 696 with the next point).
+//     That is 32768 FMAs a block and SM, 256 cycles of the fp32 pipes, and a second reader of tensor memory beside the MMAs: 0.60 us a
+//     block, where the MMAs and their copies alone take 0.44 (0.37 in the library's product of unscaled operands).
 //   * So blocks that follow one another with the same scales, as most do where A's blocks are 128 x 128 (powers of two, of
-//     weights or gradients of one kind), are multiplied into one accumulator, up to kMostJoined of them (1024 products a sum).
+//     weights or gradients of one kind), are multiplied into one accumulator, up to kMostJoined of them (1024 products a sum):
+//     12 x 4000 x 24576 x 768 in 685 us (2650 TFLOP/s), 925 where no two are equal; 8192^3 404 (2720).
+//   * Warps 2 and 3, which have no role there, bring scales, bias and tiles' coordinates to the epilogue through shared memory.
 //   * MN-major operands come in boxes of 128(MN) x 128(K): K rows of 128 B, 8-row groups 1024 B apart, boxes 16 KB apart; the
 //     32-wide K step of one MMA moves the start address by 4096 B (K-major: by 32 B).
+// What bounds it now: joined blocks, shared memory (stages written and read: 64 KB a block and SM) and, with few blocks to a tile,
+// the output's way to memory (12 x 4000 x 768 x 24576: 943 us, 740 without the copies); separate ones, the epilogue above, and for
+// few blocks its start and output between the tiles (1190 us; scales by row 1245).
+// Tried without gain: MMAs of half the columns, each half of the epilogue on its own two accumulators (925 -> 997 us); reads of 32
+// columns, packed FMAs, five stages, two stages to an MMA round.
 //
 // No TMA load uses cluster multicast.  Every wait is bounded as there.
 #pragma once
