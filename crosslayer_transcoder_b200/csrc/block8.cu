@@ -474,8 +474,9 @@ int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 // Rows that one CTA of the (Jump)ReLU kernels walks: enough CTAs for the chip, at least 8 rows (a thread's thresholds are read once).
 int rows_per_cta(int R, int C, int sms) {
   const long long across = up(up(C, 8), 256), want = up(8ll * sms, across);
-  long long rows = up(R, want);
-  return (int)(rows < 8 ? 8 : rows > 128 ? 128 : rows);
+  long long rows = up(R, want), least = up(R, 65535);  // (a grid's y)
+  rows = rows < 8 ? 8 : rows > 128 ? 128 : rows;
+  return (int)(rows < least ? least : rows);
 }
 
 template <class T>

@@ -46,13 +46,21 @@ int plan_parts(GemmGeom& g, int sms) {
     GemmGeom h = g;
     long long parts = 0;
     const long long least = up(total, room);
-    for (long long p = least < 4 ? 4 : least; p < longest; ++p) {  // (grows by the slabs' last, shorter parts: few steps)
-      h.kb_per_part = (int)p;
-      parts = 0;
-      for (int z = 0; z < g.nz; ++z) parts += part_count(h, z, kb_per_seg);
-      if (parts <= room) break;
+    if (longest * g.nz == total) {
+      const long long each = room / g.nz;  // parts of a slab
+      if (each < 2) continue;
+      h.kb_per_part = (int)(up(longest, each) < 4 ? 4 : up(longest, each));
+      parts = g.nz * up(longest, h.kb_per_part);
+    } else {
+      // (grows by the slabs' last, shorter parts: a few steps)
+      for (long long p = least < 4 ? 4 : least; p < longest; p += 1 + p / 64) {
+        h.kb_per_part = (int)p;
+        parts = 0;
+        for (int z = 0; z < g.nz; ++z) parts += part_count(h, z, kb_per_seg);
+        if (parts <= room) break;
+      }
     }
-    if (parts == 0 || parts > room || parts > 65535) continue;
+    if (parts <= g.nz || parts > room || parts > 65535) continue;
     const double us = rounds * (h.kb_per_part * block + tile) + 4.0 + 8.0 * parts * g.M * g.N / 5e6;
     if (us < best) best = us, best_part = h.kb_per_part;
   }

@@ -22,6 +22,7 @@ waits for the device first.
 """
 from __future__ import annotations
 
+import threading
 from array import array
 from typing import Optional, Sequence
 
@@ -38,6 +39,7 @@ _BATCHED, _DEC_FWD, _DEC_DFEAT, _DEC_DW = range(4)
 
 _status: Optional[torch.Tensor] = None       # one pinned word for all devices; kernels write to it only when they fail
 _status_view = None
+_status_lock = threading.Lock()
 
 
 def _blocks(n: int, rows: int = BLOCK) -> int:
@@ -49,8 +51,11 @@ def _status_word() -> torch.Tensor:
     if _status is None:
         if torch.cuda.is_current_stream_capturing():
             raise CltError("make one 8-bit call before a graph is captured: the first one allocates its status word")
-        word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        _status, _status_view = word, word.numpy()
+        with _status_lock:
+            if _status is None:
+                word = torch.zeros(1, dtype=torch.int32).pin_memory()
+                _status_view = word.numpy()
+                _status = word
     if _status_view[0] != 0:
         _raise_status("(reported by an earlier call)")
     return _status
@@ -559,6 +564,8 @@ class _JumpReLU(torch.autograd.Function):
     @_first_order
     def backward(ctx, g):
         bits, theta, bw = ctx.saved_tensors
+        if not ctx.needs_input_grad[1]:
+            theta = None                        # (where the gradient passes, the bits say by themselves)
         th = theta
         if th is not None and (th.dtype != torch.float32 or not th.is_contiguous()):
             th = th.float().contiguous()

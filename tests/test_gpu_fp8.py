@@ -371,6 +371,17 @@ def test_jump_relu_against_the_module():
     assert torch.allclose(got[1], want[1], rtol=1e-5, atol=1e-6 * float(want[1].abs().max()))
 
 
+def test_jump_relu_gradient_of_x_alone():
+    """Thresholds that need no gradient change nothing for x; so do they for many short rows."""
+    x, th, g = _rand((500, 40), 1, 0.2), torch.full((40,), 0.05, device=DEV), _rand((500, 40), 2)
+    xr, tr = x.clone().requires_grad_(), th.clone().requires_grad_()
+    want = torch.autograd.grad(fp8.jump_relu(xr, tr, 0.5), (xr, tr), g)
+    assert torch.equal(torch.autograd.grad(fp8.jump_relu(xr, th, 0.5), xr, g)[0], want[0])
+    assert torch.equal(torch.autograd.grad(fp8.jump_relu(x, tr, 0.5), tr, g)[0], want[1])
+    long = torch.randn(9_000_000, 8, device=DEV)
+    assert torch.equal(fp8.jump_relu(long), torch.relu(long))
+
+
 def test_jump_relu_strides_and_empty():
     base = _rand((30, 4, 100), 1)
     for x in (base[:, 1], base[:, :, 3:50], base[::2], base[:, 0].t(), base[0, 0].expand(9, 100), base[:0]):

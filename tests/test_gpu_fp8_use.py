@@ -195,6 +195,19 @@ def test_captured_product_of_parts():
     assert all(torch.equal(y, want) for _, y in outs)
 
 
+def test_kernel_that_a_capture_meets_first():
+    """Another type and layout than any call before: what its kernel needs is set up inside the capture."""
+    a, b = fp8.quantize(torch.randn(300, 200, device=DEV)), fp8.quantize(torch.randn(200, 136, device=DEV))
+    fp8.matmul(a, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fp8.matmul(b.mT, a.mT, out_dtype=torch.float16)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, fp8.matmul(b.mT, a.mT, out_dtype=torch.float16))
+
+
 def test_first_call_in_a_capture_is_refused(monkeypatch):
     """Nothing is allocated for the status word while a graph is being captured."""
     monkeypatch.setattr(fp8, "_status", None)
