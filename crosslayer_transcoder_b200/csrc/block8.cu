@@ -172,9 +172,10 @@ struct Source {
   __device__ __forceinline__ const void* matrix(int i, int e) const { return (const char*)x + i * z * e; }
 };
 // The decoder's blocks, tensors of their own: number t holds t + 1 matrices, one after another.
-constexpr int kMaxBlocks = 64;
+constexpr int kMaxBlocks = 361;  // as many layers as the contraction takes
+template <int kMost>
 struct BlockList {
-  const void* block[kMaxBlocks];
+  const void* block[kMost];
   long long ld, z;
   int R, C, vec;
   __device__ __forceinline__ const void* matrix(int i, int e) const {
@@ -508,13 +509,30 @@ int quantize(const Source& s, uint8_t* q, int q_ld, float* scales, float* sums, 
   return 0;
 }
 
-template <class T>
-int quantize_list(const BlockList& s, uint8_t* q, int q_ld, float* scales, int Z, cudaStream_t st) {
+template <class T, class S>
+int quantize_list(const S& s, uint8_t* q, int q_ld, float* scales, int Z, cudaStream_t st) {
   const long long rb = up(s.R, 128), cb = up(s.C, 128);
   CLT_CHECK_ARG(rb * cb < (1ll << 31), "fp8_quantize_blocks: too many blocks");
-  quantize_tile_kernel<T, false, BlockList><<<dim3((unsigned)(rb * cb), Z), 256, 0, st>>>(s, q, q_ld, scales, nullptr, (int)rb, (int)cb);
+  quantize_tile_kernel<T, false, S><<<dim3((unsigned)(rb * cb), Z), 256, 0, st>>>(s, q, q_ld, scales, nullptr, (int)rb, (int)cb);
   CLT_CHECK_CUDA(cudaGetLastError());
   return 0;
+}
+
+template <int kMost>
+int quantize_any_list(const uint64_t* blocks, int n, int in_dtype, uint8_t* q, int q_ld, float* scales, int R, int C, cudaStream_t st) {
+  const int e = elem_size(in_dtype);
+  BlockList<kMost> s{};
+  s.ld = C, s.z = (long long)R * C, s.R = R, s.C = C;
+  s.vec = (long long)C * e % 16 == 0;
+  for (int t = 0; t < n; ++t) {
+    s.block[t] = (const void*)(uintptr_t)blocks[t];
+    CLT_CHECK_ARG(s.block[t] != nullptr && blocks[t] % e == 0, "fp8_quantize_blocks: block %d is null or misaligned", t);
+    s.vec = s.vec && aligned16(s.block[t]);
+  }
+  const int Z = n * (n + 1) / 2;
+  if (in_dtype == 0) return quantize_list<float>(s, q, q_ld, scales, Z, st);
+  if (in_dtype == 1) return quantize_list<__half>(s, q, q_ld, scales, Z, st);
+  return quantize_list<__nv_bfloat16>(s, q, q_ld, scales, Z, st);
 }
 
 template <class T>
@@ -589,20 +607,9 @@ int clt_fp8_quantize_blocks(const uint64_t* blocks, int n, int in_dtype, void* q
   CLT_CHECK_ARG(in_dtype >= 0 && in_dtype <= 2, "fp8_quantize_blocks: input type %d", in_dtype);
   CLT_CHECK_ARG(q_ld >= C && q_ld % 16 == 0 && q_ld < (1ll << 31) && aligned16(q),
                 "fp8_quantize_blocks: rows of the copy must be 16-byte aligned (distance %lld)", (long long)q_ld);
-  const int e = elem_size(in_dtype);
-  BlockList s{};
-  s.ld = C, s.z = (long long)R * C, s.R = R, s.C = C;
-  s.vec = (long long)C * e % 16 == 0;
-  for (int t = 0; t < n; ++t) {
-    s.block[t] = (const void*)(uintptr_t)blocks[t];
-    CLT_CHECK_ARG(s.block[t] != nullptr && blocks[t] % e == 0, "fp8_quantize_blocks: block %d is null or misaligned", t);
-    s.vec = s.vec && aligned16(s.block[t]);
-  }
   cudaStream_t st = (cudaStream_t)stream;
-  const int Z = n * (n + 1) / 2;
-  if (in_dtype == 0) return quantize_list<float>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
-  if (in_dtype == 1) return quantize_list<__half>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
-  return quantize_list<__nv_bfloat16>(s, (uint8_t*)q, (int)q_ld, scales, Z, st);
+  return n <= 16 ? quantize_any_list<16>(blocks, n, in_dtype, (uint8_t*)q, (int)q_ld, scales, R, C, st)
+                 : quantize_any_list<kMaxBlocks>(blocks, n, in_dtype, (uint8_t*)q, (int)q_ld, scales, R, C, st);
 }
 
 int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,

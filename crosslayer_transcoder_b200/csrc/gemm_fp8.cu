@@ -185,6 +185,20 @@ int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, 
   CLT_CHECK_ARG(false, "fp8_matmul: operand layout");
 }
 
+// The 8-bit copy [Z, R, C] of a pass's operand in one buffer: values, rows of a multiple of 16, then scales of 128 x 128 blocks.
+struct Copy {
+  uint8_t* q;
+  float* s;
+  int64_t ld, z, sr, sz;  // distances of rows and matrices of the values, of rows and matrices of the scales
+  long long bytes;
+  Copy(void* buf, long long Z, long long R, long long C) {
+    ld = up(C, 16) * 16, z = R * ld, sr = up(C, 128), sz = up(R, 128) * sr;
+    q = (uint8_t*)buf;
+    s = (float*)(q + Z * z);
+    bytes = Z * (z + 4 * sz);
+  }
+};
+
 bool geom(GemmGeom& g, int mode, int M, int N, int K, int L) {
   if (mode < 0 || mode > 3 || M <= 0 || N <= 0 || K <= 0 || L <= 0 || L > (mode == kBatched ? 65535 : 361)) return false;  // slabs: a grid's y
   g = GemmGeom{mode, M, N, K, L, mode == kDecDW ? L * (L + 1) / 2 : L};
@@ -240,6 +254,81 @@ int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_tra
     }
   }
   return dispatch(g, ta, tb, fa, fb, fo, status, sms, (cudaStream_t)stream);
+}
+
+// ---- whole passes: one entry for the copies and products of a projection or a crosslayer decode --------------------------------
+int clt_fp8_copy_units(int Z, int R, int C) {
+  if (Z <= 0 || R < 0 || C <= 0) return 0;
+  const Copy c(nullptr, Z, R, C);
+  const long long n = up(c.bytes, 256);
+  return n < (1ll << 31) ? (int)n : 0;
+}
+
+int clt_fp8_pass_units(int crosslayer, int backward, int want_dx, int want_dw, int want_db, int B, int L, int K, int N) {
+  if (B <= 0 || L <= 0 || K <= 0 || N <= 0 || L > 361) return 0;
+  long long ws = 0, bytes = 0;
+  const auto parts = [&](int mode, int m, int n, int k) {
+    const long long need = 4ll * clt_fp8_matmul_parts(mode, m, n, k, L, 0) * m * n;
+    ws = need > ws ? need : ws;
+  };
+  if (!backward) {
+    parts(crosslayer ? kDecFwd : kBatched, B, N, K);
+  } else {
+    if (want_dx) parts(crosslayer ? kDecDFeat : kBatched, B, K, N);
+    if (want_dw) parts(crosslayer ? kDecDW : kBatched, K, N, B);
+    bytes = Copy(nullptr, L, B, N).bytes + (want_db ? 4ll * L * up(B, 128) * N + 256 : 0);
+  }
+  const long long n = up(bytes, 256) + up(ws, 256);
+  return n < (1ll << 31) ? (int)n : 0;
+}
+
+int clt_fp8_pass_fwd(int crosslayer, const void* x, int dtype, int64_t x_ld, int64_t x_z, const void* W, const uint64_t* blocks,
+                     int w_dtype, const float* bias, void* y, void* x_copy, void* w_copy, void* scratch, int64_t scratch_units, int B,
+                     int L, int K, int N, int* status, clt_stream_t stream) {
+  CLT_CHECK_ARG(x && (crosslayer ? (const void*)blocks : W) && y && x_copy && w_copy, "fp8_pass_fwd: null pointer");
+  CLT_CHECK_ARG(B > 0 && L > 0 && L <= 361 && K > 0 && N > 0, "fp8_pass_fwd: bad dims B=%d L=%d K=%d N=%d", B, L, K, N);
+  const Copy cx(x_copy, L, B, K), cw(w_copy, crosslayer ? L * (L + 1) / 2 : L, K, N);
+  if (int rc = clt_fp8_quantize(x, dtype, x_ld, x_z, cx.q, cx.ld, cx.s, nullptr, L, B, K, 128, stream)) return rc;
+  const int rc = crosslayer ? clt_fp8_quantize_blocks(blocks, L, w_dtype, cw.q, cw.ld, cw.s, K, N, stream)
+                            : clt_fp8_quantize(W, w_dtype, N, (int64_t)K * N, cw.q, cw.ld, cw.s, nullptr, L, K, N, 128, stream);
+  if (rc) return rc;
+  return clt_fp8_matmul(crosslayer ? kDecFwd : kBatched, cx.q, cx.ld, cx.z, 0, cx.s, cx.sz, cx.sr, 1, 128, cw.q, cw.ld, cw.z, 0, cw.s,
+                        cw.sz, 1, cw.sr, bias, N, y, dtype, (int64_t)L * N, N, (float*)scratch, scratch_units * 64, B, N, K, L, status,
+                        stream);
+}
+
+int clt_fp8_pass_bwd(int crosslayer, const void* g, int dtype, int64_t g_ld, int64_t g_z, const void* x_copy, const void* w_copy,
+                     void* dx, void* dW, int w_dtype, float* db, void* scratch, int64_t scratch_units, int B, int L, int K, int N,
+                     int* status, clt_stream_t stream) {
+  CLT_CHECK_ARG(g && scratch && (!dx || w_copy) && (!dW || x_copy), "fp8_pass_bwd: null pointer");
+  CLT_CHECK_ARG(B > 0 && L > 0 && L <= 361 && K > 0 && N > 0, "fp8_pass_bwd: bad dims B=%d L=%d K=%d N=%d", B, L, K, N);
+  CLT_CHECK_ARG((uintptr_t)scratch % 16 == 0 &&
+                    scratch_units >= clt_fp8_pass_units(crosslayer, 1, dx != nullptr, dW != nullptr, db != nullptr, B, L, K, N),
+                "fp8_pass_bwd: scratch is misaligned or too small (%lld units)", (long long)scratch_units);
+  const Copy cg(scratch, L, B, N);
+  const int chunks = (int)up(B, 128);
+  float* part = db ? (float*)((uint8_t*)scratch + up(cg.bytes, 256) * 256) : nullptr;
+  const long long used = up(cg.bytes + (db ? 4ll * L * chunks * N + 256 : 0), 256);
+  float* ws = (float*)((uint8_t*)scratch + used * 256);
+  const int64_t ws_floats = (scratch_units - used) * 64;
+  if (int rc = clt_fp8_quantize(g, dtype, g_ld, g_z, cg.q, cg.ld, cg.s, part, L, B, N, 128, stream)) return rc;
+  if (db)
+    if (int rc = clt_sum_chunks(part, db, L, chunks, N, stream)) return rc;
+  if (dx) {
+    const Copy cw(const_cast<void*>(w_copy), crosslayer ? L * (L + 1) / 2 : L, K, N);
+    if (int rc = clt_fp8_matmul(crosslayer ? kDecDFeat : kBatched, cg.q, cg.ld, cg.z, 0, cg.s, cg.sz, cg.sr, 1, 128, cw.q, cw.ld, cw.z,
+                                1, cw.s, cw.sz, cw.sr, 1, nullptr, 0, dx, dtype, (int64_t)L * K, K, ws, ws_floats, B, K, N, L, status,
+                                stream))
+      return rc;
+  }
+  if (dW) {
+    const Copy cx(const_cast<void*>(x_copy), L, B, K);
+    if (int rc = clt_fp8_matmul(crosslayer ? kDecDW : kBatched, cx.q, cx.ld, cx.z, 1, cx.s, cx.sz, 1, cx.sr, 128, cg.q, cg.ld, cg.z, 0,
+                                cg.s, cg.sz, 1, cg.sr, nullptr, 0, dW, w_dtype, N, (int64_t)K * N, ws, ws_floats, K, N, B, L, status,
+                                stream))
+      return rc;
+  }
+  return 0;
 }
 
 }  // extern "C"

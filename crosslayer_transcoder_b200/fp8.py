@@ -183,18 +183,6 @@ def _dequantize(v, s, block_rows, dtype):
     return out
 
 
-def _quantize(x, x_ld: int, x_z: int, Z: int, R: int, C: int, block_rows: int, v, s, sums=None):
-    """x (rows x_ld apart, matrices x_z) to the values v [Z, R, pitch] and scales s; ``sums [Z, C]``: its column sums."""
-    if Z * R * C == 0:
-        if sums is not None:
-            sums.zero_()
-        return
-    part = None if sums is None else torch.empty(Z, _blocks(R), C, dtype=torch.float32, device=x.device)
-    lib().call("clt_fp8_quantize", x, DTYPE_CODE[x.dtype], x_ld, x_z, v, _pitch(C), s, part, Z, R, C, block_rows, stream_ptr())
-    if part is not None:
-        lib().call("clt_sum_chunks", part, sums, Z, _blocks(R), C, stream_ptr())
-
-
 def _quantize_any(x, block_rows):
     """quantize of a matrix or a stack."""
     if x.stride(-1) != 1 and x.shape[-1] > 1:
@@ -204,7 +192,9 @@ def _quantize_any(x, block_rows):
     Z, x_z = (shape[0], x.stride(0)) if len(shape) == 3 else (1, 0)
     v = _storage(*shape, device=x.device)
     s = torch.empty(*shape[:-2], _blocks(R, block_rows), _blocks(C), dtype=torch.float32, device=x.device)
-    _quantize(x, x.stride(-2), x_z, Z, R, C, block_rows, v, s)
+    if x.numel():
+        lib().call("clt_fp8_quantize", x, DTYPE_CODE[x.dtype], x.stride(-2), x_z, v, _pitch(C), s, None, Z, R, C, block_rows,
+                   stream_ptr())
     return BlockTensor._of(v, s, block_rows)
 
 
@@ -300,70 +290,56 @@ def matmul(a: BlockTensor, b: BlockTensor, bias: Optional[torch.Tensor] = None,
 
 
 # ---- differentiable passes ------------------------------------------------------------------------------------------------------
-class _Copy:
-    """Where the 8-bit copy [Z, R, C] of a pass's operand is: one buffer, its values first, then its scales."""
-
-    __slots__ = ("buf", "Z", "R", "C", "at")
-
-    def __init__(self, Z, R, C, device=None, buf=None):
-        self.Z, self.R, self.C = Z, R, C
-        self.at = (Z * R * _pitch(C) + 3) & ~3              # bytes before the scales
-        self.buf = buf if buf is not None else \
-            torch.empty(self.at + 4 * Z * _blocks(R) * _blocks(C), dtype=torch.uint8, device=device)
-
-    def fill(self, x, x_ld, x_z, first=0, count=None, sums=None):
-        """Matrices first .. first + count from x."""
-        count = self.Z if count is None else count
-        p = self.buf.data_ptr()
-        _quantize(x, x_ld, x_z, count, self.R, self.C, BLOCK, p + first * self.R * _pitch(self.C),
-                  p + self.at + 4 * first * _blocks(self.R) * _blocks(self.C), sums)
-        return self
-
-    def operand(self, rows_are_k: bool, transposed: bool):
-        p, ld, rb, cb = self.buf.data_ptr(), _pitch(self.C), _blocks(self.R), _blocks(self.C)
-        return p, ld, self.R * ld, int(transposed), p + self.at, rb * cb, *((1, cb) if rows_are_k else (cb, 1))
+_BYTES = dict(dtype=torch.uint8)
 
 
 def _rows_first(x):
     """x [B, L, C] with unit distance inside a row: (x, distance of rows, distance of layers)."""
+    if x.is_contiguous():
+        return x, x.shape[1] * x.shape[2], x.shape[2]
     if x.stride(2) != 1 and x.shape[2] > 1:
         x = x.contiguous()
     return x, x.stride(0), x.stride(1)
 
 
-def _project_forward(x, W, b, keep_x, keep_w):
-    B, L, D = x.shape
-    F = W.shape[2]
-    y = torch.empty(B, L, F, dtype=x.dtype, device=x.device)
-    xc = _Copy(L, B, D, x.device).fill(*_rows_first(x))
-    if W.stride(2) != 1:
-        W = W.contiguous()
-    wc = _Copy(L, D, F, x.device).fill(W, W.stride(1), W.stride(0))
+def _pass_forward(crosslayer, x, W, blocks, w_dtype, b, N):
+    """y [B, L, N] and the 8-bit copies of x [B, L, K] and of the weights (``W``, or the addresses of a decoder's ``blocks``)."""
+    status, call, query, dev = _status_word(), lib().call, lib().query, x.device
+    B, L, K = x.shape
+    y = torch.empty(B, L, N, dtype=x.dtype, device=dev)
+    x_copy = torch.empty(256 * query("clt_fp8_copy_units", L, B, K), device=dev, **_BYTES)
+    w_copy = torch.empty(256 * query("clt_fp8_copy_units", _pairs(L) if crosslayer else L, K, N), device=dev, **_BYTES)
     if B:
-        b = None if b is None else b.detach().float().contiguous()
-        _contract(_BATCHED, xc.operand(False, False), wc.operand(True, False), b, F, y, L * F, F, B, F, D, L)
-    return y, xc.buf if keep_x else None, wc.buf if keep_w else None
+        n = query("clt_fp8_pass_units", crosslayer, 0, 0, 0, 0, B, L, K, N)
+        scratch = torch.empty(256 * n, device=dev, **_BYTES) if n else None
+        x, ld, z = _rows_first(x)
+        if b is not None and (b.dtype != torch.float32 or not b.is_contiguous()):
+            b = b.float().contiguous()
+        code = DTYPE_CODE[x.dtype]
+        call("clt_fp8_pass_fwd", crosslayer, x, code, ld, z, W, blocks, DTYPE_CODE[w_dtype], b, y, x_copy, w_copy, scratch, n, B, L, K,
+             N, status, stream_ptr())
+    return y, x_copy, w_copy
 
 
-def _project_backward(g, x_buf, w_buf, dims, types, need):
-    B, L, D, F = dims
-    dev = g.device
-    dx = dW = None
-    db = torch.empty(L, F, dtype=torch.float32, device=dev) if need[2] else None
-    gc = _Copy(L, B, F, dev).fill(*_rows_first(g), sums=db)
-    if need[0]:
-        dx = torch.empty(B, L, D, dtype=types[0], device=dev)
-        if B:
-            _contract(_BATCHED, gc.operand(False, False), _Copy(L, D, F, buf=w_buf).operand(False, True), None, 0, dx, L * D, D,
-                      B, D, F, L)
-    if need[1]:
-        dW = torch.empty(L, D, F, dtype=types[1], device=dev)
-        if B:
-            _contract(_BATCHED, _Copy(L, B, D, buf=x_buf).operand(True, True), gc.operand(True, False), None, 0, dW, F, D * F,
-                      D, F, B, L)
-        else:
-            dW.zero_()
-    return dx, dW, db if db is None or types[2] == torch.float32 else db.to(types[2])
+def _pass_backward(crosslayer, g, x_copy, w_copy, K, x_dtype, w_dtype, need_x, need_w, need_b):
+    """(dx [B, L, K], dW [L or pairs, K, N], db [L, N]), None for what is not needed."""
+    status, dev = _status_word(), g.device
+    B, L, N = g.shape
+    new = torch.empty if B else torch.zeros
+    dx = new(B, L, K, dtype=x_dtype, device=dev) if need_x else None
+    dW = new(_pairs(L) if crosslayer else L, K, N, dtype=w_dtype, device=dev) if need_w else None
+    db = new(L, N, dtype=torch.float32, device=dev) if need_b else None
+    if B:
+        n = lib().query("clt_fp8_pass_units", crosslayer, 1, need_x, need_w, need_b, B, L, K, N)
+        scratch = torch.empty(256 * n, device=dev, **_BYTES)
+        g, ld, z = _rows_first(g)
+        lib().call("clt_fp8_pass_bwd", crosslayer, g, DTYPE_CODE[g.dtype], ld, z, x_copy, w_copy, dx, dW, DTYPE_CODE[w_dtype], db,
+                   scratch, n, B, L, K, N, status, stream_ptr())
+    return dx, dW, db
+
+
+def _pairs(t: int) -> int:
+    return t * (t + 1) // 2
 
 
 class _Project(torch.autograd.Function):
@@ -372,25 +348,30 @@ class _Project(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b):
         need_x, need_w = ctx.needs_input_grad[:2]
-        shapes = x.shape, W.shape, None if b is None else b.shape
-        if W.dim() == 2:
-            W = W.unsqueeze(0)
-        L, D, F = W.shape
-        out_shape = (*x.shape[:-1], F)
-        x = x.reshape(shapes[0].numel() // (L * D), L, D)
-        y, x_buf, w_buf = _on(x.device, _project_forward, x, W, b, need_w, need_x)
-        ctx.dims, ctx.shapes = (x.shape[0], L, D, F), shapes
+        ctx.shapes = xs, ws, _ = x.shape, W.shape, None if b is None else b.shape
         ctx.types = x.dtype, W.dtype, None if b is None else b.dtype
-        ctx.save_for_backward(x_buf, w_buf)
-        return y.view(out_shape)
+        L, (K, N) = 1 if len(ws) == 2 else ws[0], ws[-2:]
+        if len(ws) == 2 or len(xs) != 3:
+            x = x.reshape(xs.numel() // (L * K), L, K)
+        if not W.is_contiguous():
+            W = W.contiguous()
+        y, x_copy, w_copy = _on(x.device, _pass_forward, 0, x, W, None, W.dtype, b, N)
+        ctx.dims = x.shape[0], L, K, N
+        ctx.save_for_backward(x_copy if need_w else None, w_copy if need_x else None)
+        return y if len(xs) == 3 and len(ws) == 3 else y.view(*xs[:-1], N)
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
-        B, L, D, F = ctx.dims
-        dx, dW, db = _on(g.device, _project_backward, g.reshape(B, L, F), *ctx.saved_tensors, ctx.dims, ctx.types,
-                         ctx.needs_input_grad)
+        B, L, K, N = ctx.dims
         xs, ws, bs = ctx.shapes
+        x_copy, w_copy = ctx.saved_tensors
+        dx, dW, db = _on(g.device, _pass_backward, 0, g.reshape(B, L, N), x_copy, w_copy, K, ctx.types[0], ctx.types[1],
+                         *ctx.needs_input_grad)
+        if db is not None and ctx.types[2] != torch.float32:
+            db = db.to(ctx.types[2])
+        if len(xs) == 3 and len(ws) == 3:
+            return dx, dW, db
         return (None if dx is None else dx.view(xs), None if dW is None else dW.view(ws), None if db is None else db.view(bs))
 
 
@@ -403,6 +384,8 @@ def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) 
     _check("W", W, DTYPE_CODE, x.device)
     ws, xs = W.shape, x.shape
     one = len(ws) == 2
+    if not one and len(ws) == 3 and ws[0] > 361:
+        raise ValueError(f"{ws[0]} layers: at most 361 are supported")
     if len(ws) not in (2, 3) or W.numel() == 0:
         raise ValueError(f"expected W [D, F] or [L, D, F], not empty, got {tuple(ws)}")
     inner = 1 if one else 2
@@ -415,74 +398,38 @@ def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) 
     return _Project.apply(x, W, b)
 
 
-def _pairs(t: int) -> int:
-    return t * (t + 1) // 2
-
-
-def _decode_forward(f, b, blocks, keep_f, keep_w):
-    B, L, F = f.shape
-    D = blocks[0].shape[2]
-    y = torch.empty(B, L, D, dtype=f.dtype, device=f.device)
-    fc = _Copy(L, B, F, f.device).fill(*_rows_first(f))
-    wc = _Copy(_pairs(L), F, D, f.device)
-    if L <= 64 and all(w.is_contiguous() and w.dtype == blocks[0].dtype for w in blocks):
-        at = array("Q", [w.data_ptr() for w in blocks])
-        p = wc.buf.data_ptr()
-        lib().call("clt_fp8_quantize_blocks", at.buffer_info()[0], L, DTYPE_CODE[blocks[0].dtype], p, _pitch(D), p + wc.at, F, D,
-                   stream_ptr())
-    else:
-        for t, w in enumerate(blocks):
-            if w.stride(2) != 1:
-                w = w.contiguous()
-            wc.fill(w, w.stride(1), w.stride(0), first=_pairs(t), count=t + 1)
-    if B:
-        b = None if b is None else b.detach().float().contiguous()
-        _contract(_DEC_FWD, fc.operand(False, False), wc.operand(True, False), b, D, y, L * D, D, B, D, F, L)
-    return y, fc.buf if keep_f else None, wc.buf if keep_w else None
-
-
-def _decode_backward(g, f_buf, w_buf, dims, types, need):
-    B, L, F, D = dims
-    dev = g.device
-    df, dW = None, [None] * L
-    db = torch.empty(L, D, dtype=torch.float32, device=dev) if need[1] else None
-    gc = _Copy(L, B, D, dev).fill(*_rows_first(g), sums=db)
-    if need[0]:
-        df = torch.empty(B, L, F, dtype=types[0], device=dev)
-        if B:
-            _contract(_DEC_DFEAT, gc.operand(False, False), _Copy(_pairs(L), F, D, buf=w_buf).operand(False, True), None, 0, df,
-                      L * F, F, B, F, D, L)
-    if any(need[2:]):
-        flat = torch.empty(_pairs(L), F, D, dtype=torch.float32, device=dev)
-        if B:
-            _contract(_DEC_DW, _Copy(L, B, F, buf=f_buf).operand(True, True), gc.operand(True, False), None, 0, flat, D, F * D,
-                      F, D, B, L)
-        else:
-            flat.zero_()
-        dW = [flat[_pairs(t):_pairs(t + 1)].to(types[2][t]) if need[2 + t] else None for t in range(L)]
-    return (df, db if db is None or types[1] == torch.float32 else db.to(types[1]), *dW)
-
-
 class _CrosslayerDecode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, f, b, *blocks):
         need_w = any(ctx.needs_input_grad[2:])
-        ctx.shape = f.shape
-        L, F, D = *f.shape[-2:], blocks[0].shape[2]
-        f = f.reshape(f.numel() // (L * F), L, F)
-        y, f_buf, w_buf = _on(f.device, _decode_forward, f, b, blocks, need_w, ctx.needs_input_grad[0])
-        ctx.dims = f.shape[0], L, F, D
+        shape = ctx.shape = f.shape
         ctx.types = f.dtype, None if b is None else b.dtype, [w.dtype for w in blocks]
-        ctx.save_for_backward(f_buf, w_buf)
-        return y.view(*ctx.shape[:-1], D)
+        (L, F), D = shape[-2:], blocks[0].shape[2]
+        if len(shape) != 3:
+            f = f.reshape(shape.numel() // (L * F), L, F)
+        dtype = blocks[0].dtype
+        if not all(w.dtype == dtype and w.is_contiguous() for w in blocks):
+            dtype = torch.float32
+            blocks = [w.float().contiguous() for w in blocks]
+        at = array("Q", [w.data_ptr() for w in blocks])
+        y, f_copy, w_copy = _on(f.device, _pass_forward, 1, f, None, at.buffer_info()[0], dtype, b, D)
+        ctx.dims = f.shape[0], L, F, D
+        ctx.save_for_backward(f_copy if need_w else None, w_copy if ctx.needs_input_grad[0] else None)
+        return y if len(shape) == 3 else y.view(*shape[:-1], D)
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
         B, L, F, D = ctx.dims
-        df, *rest = _on(g.device, _decode_backward, g.reshape(B, L, D), *ctx.saved_tensors, ctx.dims, ctx.types,
-                        ctx.needs_input_grad)
-        return (None if df is None else df.view(ctx.shape), *rest)
+        need_f, need_b, *need_w = ctx.needs_input_grad
+        f_copy, w_copy = ctx.saved_tensors
+        f_type, b_type, w_types = ctx.types
+        same = w_types[0] if all(t == w_types[0] for t in w_types) else torch.float32
+        df, dW, db = _on(g.device, _pass_backward, 1, g.reshape(B, L, D), f_copy, w_copy, F, f_type, same, need_f, any(need_w), need_b)
+        if db is not None and b_type != torch.float32:
+            db = db.to(b_type)
+        parts = [dW[_pairs(t):_pairs(t + 1)].to(w_types[t]) if need else None for t, need in enumerate(need_w)]
+        return (None if df is None else df.view(ctx.shape), db, *parts)
 
 
 def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -494,6 +441,8 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
     if len(shape) < 2 or shape[-2] == 0 or len(blocks) != shape[-2]:
         raise ValueError(f"{len(blocks)} decoder blocks do not match features {tuple(shape)}")
     L, F = shape[-2:]
+    if L > 361:
+        raise ValueError(f"{L} layers: at most 361 are supported")
     for t, w in enumerate(blocks):
         _check(f"blocks[{t}]", w, DTYPE_CODE, features.device)
         if w.shape != (t + 1, F, blocks[0].shape[-1]) or w.numel() == 0:

@@ -490,7 +490,7 @@ int clt_cast_bf16(const float* src, void* dst, int64_t n, clt_stream_t stream);
 int clt_fp8_quantize(const void* x, int in_dtype, int64_t ld, int64_t z_stride, void* q, int64_t q_ld, float* scales,
                      float* column_sums, int Z, int R, int C, int block_rows, clt_stream_t stream);
 int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_stream_t stream);
-/* clt_fp8_quantize by blocks of 128 x 128 of the decoder's tensors, n <= 64 of them: blocks[t] (a host array of device addresses) is a
+/* clt_fp8_quantize by blocks of 128 x 128 of the decoder's tensors, n <= 361 of them: blocks[t] (a host array of device addresses) is a
  * contiguous [t + 1, R, C]; q and scales take their n (n + 1) / 2 matrices one after another. */
 int clt_fp8_quantize_blocks(const uint64_t* blocks, int n, int in_dtype, void* q, int64_t q_ld, float* scales, int R, int C,
                             clt_stream_t stream);
@@ -516,6 +516,22 @@ int clt_fp8_matmul(int mode, const void* a, int64_t a_ld, int64_t a_z, int a_tra
                    int out_dtype, int64_t out_ld, int64_t out_z, float* ws, int64_t ws_floats, int M, int N, int K, int L,
                    int* status, clt_stream_t stream);
 int clt_fp8_matmul_parts(int mode, int M, int N, int K, int L, int num_sms);
+
+/* A whole pass and its backward.  crosslayer == 0: y [B, L, N] = x [B, L, K] W [L, K, N] + bias [L, N], layer by layer (Encoder.forward,
+ * Decoder.forward); 1: y[b, t] = sum_{s<=t} x[b, s] blocks[t][s] + bias[t] (CrosslayerDecoder.forward), blocks as in
+ * clt_fp8_quantize_blocks.  L <= 361.  x and y have type dtype; rows of x are x_ld apart, layers x_z; bias may be NULL.  x_copy and
+ * w_copy take the operands in 8 bits, by blocks of 128 x 128: clt_fp8_copy_units(L, B, K) and (L or L (L + 1) / 2, K, N) units of 256
+ * bytes, 16-byte aligned.  Backward reads them: dx [B, L, K] in dtype (NULL: not wanted, w_copy is not read), dW [L or pairs, K, N] in
+ * w_dtype (NULL: x_copy is not read), db [L, N] (may be NULL) from g [B, L, N].  scratch: clt_fp8_pass_units units of 256 bytes; forward
+ * does with less, then without parts.  The functions that count units launch nothing. */
+int clt_fp8_copy_units(int Z, int R, int C);
+int clt_fp8_pass_units(int crosslayer, int backward, int want_dx, int want_dw, int want_db, int B, int L, int K, int N);
+int clt_fp8_pass_fwd(int crosslayer, const void* x, int dtype, int64_t x_ld, int64_t x_z, const void* W, const uint64_t* blocks,
+                     int w_dtype, const float* bias, void* y, void* x_copy, void* w_copy, void* scratch, int64_t scratch_units, int B,
+                     int L, int K, int N, int* status, clt_stream_t stream);
+int clt_fp8_pass_bwd(int crosslayer, const void* g, int dtype, int64_t g_ld, int64_t g_z, const void* x_copy, const void* w_copy,
+                     void* dx, void* dW, int w_dtype, float* db, void* scratch, int64_t scratch_units, int B, int L, int K, int N,
+                     int* status, clt_stream_t stream);
 
 /* JumpReLU (theta [C]) or ReLU (theta NULL) of x [R, C] (rows ld apart; crosslayer_transcoder/model/jumprelu.py:17-48) with a
  * checkpoint of two bits a value instead of x: y [R, C] = x where x > theta and x > 0, else 0 (NaN stays NaN); bits: ceil(C / 8)

@@ -47,6 +47,7 @@ def _block(R=256, C=256, rows=128, Z=None):
     (lambda: fp8.crosslayer_decode(torch.zeros(5, 2, 4), [torch.zeros(1, 4, 3), torch.zeros(2, 4, 2)]), ValueError),
     (lambda: fp8.crosslayer_decode(torch.zeros(5, 1, 4), [torch.zeros(1, 4, 3)], torch.zeros(3)), ValueError),
     (lambda: fp8.crosslayer_decode(torch.zeros(5, 0, 4), []), ValueError),
+    (lambda: fp8.project(torch.zeros(1, 362, 1), torch.zeros(362, 1, 1)), ValueError),
     (lambda: fp8.jump_relu(torch.tensor(1.0)), ValueError),
     (lambda: fp8.jump_relu(torch.zeros(3, 4), torch.zeros(3)), ValueError),
     (lambda: fp8.jump_relu(torch.zeros(4), torch.zeros(2, 4)), ValueError),
@@ -101,6 +102,15 @@ def test_parts_cover_the_contraction(mode, M, N, K, L):
     assert lib().query("clt_fp8_matmul_parts", mode, M, N, 0, L, 148) == 0
 
 
+@pytest.mark.parametrize("Z, R, C", [(1, 1, 1), (3, 136, 64), (12, 4000, 10000), (2, 129, 257)])
+def test_copies_have_room(Z, R, C):
+    """A copy's buffer holds its values, rows of a multiple of 16, and the scales of its blocks, and not 256 bytes more."""
+    need = Z * R * (-(-C // 16) * 16) + 4 * Z * -(-R // 128) * -(-C // 128)
+    units = lib().query("clt_fp8_copy_units", Z, R, C)
+    assert need <= 256 * units < need + 256
+    assert lib().query("clt_fp8_copy_units", Z, 0, C) == 0
+
+
 def test_status_word(monkeypatch):
     """What a kernel reports reaches the next call, once."""
     word = torch.zeros(1, dtype=torch.int32)
@@ -126,7 +136,7 @@ def test_library_refuses():
     with pytest.raises(CltError, match="misaligned"):
         call("clt_fp8_quantize", p + 2, 0, 128, 0, p, 128, p, None, 1, 1, 128, 1, None)
     one = torch.tensor([0], dtype=torch.int64)          # a host array with a null address
-    for n, text in ((0, "bad dims"), (65, "bad dims"), (1, "null")):
+    for n, text in ((0, "bad dims"), (362, "bad dims"), (1, "null")):
         with pytest.raises(CltError, match=text):
             call("clt_fp8_quantize_blocks", one, n, 0, p, 128, p, 4, 128, None)
     with pytest.raises(CltError, match="null"):
@@ -150,5 +160,19 @@ def test_library_refuses():
         call("clt_jump_relu_bwd", p, 8, p, p, None, 1.0, p, None, None, 0, 0, 1, 8, None)
     with pytest.raises(CltError, match="scratch"):
         call("clt_jump_relu_bwd", p, 8, p, p, None, 1.0, p, p, p, 3, 0, 1, 8, None)
+    fwd = [0, p, 0, 64, 64, p, None, 0, None, p, p, p, None, 0, 4, 1, 64, 64, p, None]
+    for at, value, text in ((1, None, "null"), (5, None, "null"), (9, None, "null"), (0, 1, "null"), (14, 0, "bad dims"), (15, 362, "bad dims"),
+                            (10, p + 8, "16-byte")):
+        bad = list(fwd)
+        bad[at] = value
+        with pytest.raises(CltError, match=text):
+            call("clt_fp8_pass_fwd", *bad)
+    bwd = [0, p, 0, 64, 64, p, p, p, p, 0, p, p, 1 << 20, 4, 1, 64, 64, p, None]
+    for at, value, text in ((1, None, "null"), (5, None, "null"), (6, None, "null"), (11, None, "null"), (12, 1, "too small"), (11, p + 4, "misaligned"),
+                            (16, 0, "bad dims")):
+        bad = list(bwd)
+        bad[at] = value
+        with pytest.raises(CltError, match=text):
+            call("clt_fp8_pass_bwd", *bad)
     with pytest.raises(CltError, match="bad dims"):
         call("clt_sum_chunks", p, p, 0, 1, 8, None)
