@@ -32,6 +32,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "gemm_tc.cuh"
 
 namespace clt {
@@ -81,6 +83,7 @@ struct alignas(16) ScaleRing {
 constexpr int kSmemBytes =
     kOperandBytes + kEpiWarps * kOutBytes + 1024 /*alignment slack*/ + 256 /*barriers*/ + (int)sizeof(ScaleRing<true>);
 static_assert(sizeof(tc::Barriers) <= 256 && sizeof(ScaleRing<false>) <= sizeof(ScaleRing<true>) && kSmemBytes <= 232448, "shared memory");
+constexpr int kRowsOut = 4;    // rows of the output in flight where they are written value by value
 constexpr int kScaleWarps = 2;  // warps 2 and 3
 
 // Scales of one operand: element strides between matrices, between blocks along M (or N) and along K.
@@ -264,22 +267,31 @@ __device__ __forceinline__ void store_warp(const float (&acc)[128], uint8_t* buf
       }
     } else {
       __syncwarp();
+      // a few rows at a time, so that their reads and stores are in flight together (one by one: 25 us of products took 61 to
+      // 66, now 25 to 32; more rows spill)
+      using U = typename std::conditional<kOut == 0, uint32_t, uint16_t>::type;
       const int rows = min(32, M - row0);
 #pragma unroll
-      for (int c = c0; c < c0 + 2; ++c) {
-        const int n = col0 + c * kCols, cols = min(kCols, N - n);
-        uint8_t* p = (uint8_t*)o.p + (z * o.z + (long long)row0 * o.ld + n) * kSize;
+      for (int j = 0; j < 2 * kCols; j += 32) {
+        const int col = c0 * kCols + j + lane, k = (j + lane) % kCols;
+        U* p = (U*)o.p + z * o.z + (long long)row0 * o.ld + col0 + col;
+        const uint8_t* box = buf + (j + lane) / kCols * 4096 + k % kPer * kSize;
+        if (col0 + col < N) {
 #pragma unroll 1
-        for (int r = 0; r < rows; ++r) {
+          for (int r0 = 0; r0 < rows; r0 += kRowsOut) {
+            U v[kRowsOut];
 #pragma unroll
-          for (int k = lane; k < kCols; k += 32) {
-            if (k < cols) {
-              const uint8_t* v = buf + (c & 1) * 4096 + r * 128 + (((k / kPer) ^ (r & 7)) << 4) + k % kPer * kSize;
-              if constexpr (kOut == 0)
-                *reinterpret_cast<uint32_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint32_t*>(v);
-              else
-                *reinterpret_cast<uint16_t*>(p + (r * o.ld + k) * kSize) = *reinterpret_cast<const uint16_t*>(v);
+            for (int r = 0; r < kRowsOut; ++r)
+              v[r] = *reinterpret_cast<const U*>(box + (r0 + r) * 128 + (((k / kPer) ^ ((r0 + r) & 7)) << 4));
+            if (r0 + kRowsOut <= rows) {
+#pragma unroll
+              for (int r = 0; r < kRowsOut; ++r) p[r * o.ld] = v[r];
+            } else {
+#pragma unroll
+              for (int r = 0; r < kRowsOut; ++r)
+                if (r0 + r < rows) p[r * o.ld] = v[r];
             }
+            p += kRowsOut * o.ld;
           }
         }
       }
