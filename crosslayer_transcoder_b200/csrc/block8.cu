@@ -359,6 +359,32 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
   for (int h = 0; h < 2; ++h) store8<T>(o + 8 * h, left - 8 * h, out_vec && left >= 8 * h + 8, f[h]);
 }
 
+// Rows of bytes that start anywhere, to rows that start on 16 bytes: 16 of them to a thread, joined of five aligned words (bytes, at
+// the matrix's ends).
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restrict__ q, long long q_ld, long long q_z,
+                                                         uint8_t* __restrict__ out, int pitch, int R, int C, unsigned groups, long long n) {
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i >= n) return;
+  const long long row = i / groups;
+  const int c = (int)(i - row * groups) * 16;
+  const long long z = row / R;
+  const uint8_t *begin = q + z * q_z, *end = begin + (R - 1) * q_ld + C, *p = begin + (row - z * R) * q_ld + c;
+  const uint8_t* from = (const uint8_t*)((uintptr_t)p & ~(uintptr_t)3);
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (from >= begin && from + 20 <= end) {
+    uint32_t v[5];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) v[k] = reinterpret_cast<const uint32_t*>(from)[k];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(v[k], v[k + 1], 8 * ((uintptr_t)p & 3));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (c + k < C) w[k >> 2] |= (uint32_t)p[k] << 8 * (k & 3);
+  }
+  *reinterpret_cast<uint4*>(out + row * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct Bandwidth {
   const float* p;  // on the device, or NULL for
   float value;
@@ -624,6 +650,19 @@ int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* sc
   if (out_dtype == 0) return dequantize<float>((const uint8_t*)q, q_ld, q_z, sc, (float*)out, Z, R, C, st);
   if (out_dtype == 1) return dequantize<__half>((const uint8_t*)q, q_ld, q_z, sc, (__half*)out, Z, R, C, st);
   return dequantize<__nv_bfloat16>((const uint8_t*)q, q_ld, q_z, sc, (__nv_bfloat16*)out, Z, R, C, st);
+}
+
+int clt_fp8_align(const void* q, int64_t q_ld, int64_t q_z, void* out, int64_t pitch, int Z, int R, int C, clt_stream_t stream) {
+  CLT_CHECK_ARG(q && out, "fp8_align: null pointer");
+  CLT_CHECK_ARG(Z > 0 && R > 0 && C > 0 && q_ld >= 0 && q_z >= 0, "fp8_align: bad dims Z=%d R=%d C=%d", Z, R, C);
+  CLT_CHECK_ARG(pitch >= C && pitch % 16 == 0 && pitch < (1ll << 31) && aligned16(out),
+                "fp8_align: rows of the result must be 16-byte aligned (distance %lld)", (long long)pitch);
+  const long long groups = up(C, 16), n = (long long)Z * R * groups, grid = up(n, 256);
+  CLT_CHECK_ARG(grid < (1ll << 31), "fp8_align: too many values");
+  align_rows_kernel<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)q, q_ld, q_z, (uint8_t*)out, (int)pitch, R, C,
+                                                                      (unsigned)groups, n);
+  CLT_CHECK_CUDA(cudaGetLastError());
+  return 0;
 }
 
 int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_stream_t stream) {

@@ -222,8 +222,11 @@ def _operand(v: torch.Tensor, s: torch.Tensor, rows_are_k: bool, transposed: boo
     if R == 1:
         ld = _pitch(C)
     if (v.stride(-1) != 1 and C > 1) or ld % 16 or ld < C or v.data_ptr() % 16 or (Z > 1 and (z % 16 or z <= 0)):
-        copy = _storage(*v.shape, device=v.device)
-        copy.view(torch.uint8).copy_(v.view(torch.uint8))
+        if v.stride(-1) != 1 and C > 1:
+            v = v.contiguous()
+            z = v.stride(0) if stack else 0
+        copy = torch.empty(*v.shape[:-1], _pitch(C), dtype=torch.uint8, device=v.device)
+        lib().call("clt_fp8_align", v, v.stride(-2), z, copy, _pitch(C), Z, R, C, stream_ptr())
         v, ld, z = copy, _pitch(C), R * _pitch(C)
     sr, sc = s.stride(-2), s.stride(-1)
     return v, ld, z, int(transposed), s, s.stride(0) if stack else 0, *((sc, sr) if rows_are_k else (sr, sc))

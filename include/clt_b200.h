@@ -499,6 +499,8 @@ int clt_fp8_quantize_blocks(const uint64_t* blocks, int n, int in_dtype, void* q
 int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* scales, int64_t s_z, int64_t s_r, int64_t s_c,
                        int block_rows, void* out, int out_dtype, int Z, int R, int C, clt_stream_t stream);
 
+/* Values q [Z, R, C] (any distances) to out [Z, R, pitch], 16-byte aligned with pitch a multiple of 16, as clt_fp8_matmul reads them. */
+int clt_fp8_align(const void* q, int64_t q_ld, int64_t q_z, void* out, int64_t pitch, int Z, int R, int C, clt_stream_t stream);
 /* out[z] = A B + bias[z] over slabs z, in fp32 sums, rounded once to out_dtype.  A [M, K] (a_trans: stored [K, M]) with blocks of
  * a_rows x 128 (a_trans: 128 x 128), B [K, N] (b_trans: stored [N, K]) with blocks of 128 x 128; a_mn / a_k: distances of the
  * scales between blocks along M and along K, likewise for B along N and K.  Any fp32 scales will do whose products are finite.

@@ -139,6 +139,8 @@ def test_library_refuses():
     for n, text in ((0, "bad dims"), (362, "bad dims"), (1, "null")):
         with pytest.raises(CltError, match=text):
             call("clt_fp8_quantize_blocks", one, n, 0, p, 128, p, 4, 128, None)
+    with pytest.raises(CltError, match="16-byte aligned"):
+        call("clt_fp8_align", p, 100, 0, p, 100, 1, 1, 100, None)
     with pytest.raises(CltError, match="null"):
         call("clt_fp8_dequantize", None, 128, 0, p, 1, 1, 1, 1, p, 0, 1, 1, 128, None)
     with pytest.raises(CltError, match="output type"):

@@ -147,6 +147,26 @@ def test_matmul_any_scales_and_strides():
     assert torch.equal(a.dequantize().cpu(), (va[:, 2:K + 2].float() * sa.repeat_interleave(128, 1)[:, :K]))
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 1, 17), (2, 3, 15), (3, 5, 129), (1, 40, 333), (2, 129, 1001)])
+@pytest.mark.parametrize("start", [0, 1, 2, 3, 7])
+def test_matmul_rows_that_start_anywhere(shape, start):
+    """Values without a gap between rows, from any address, broadcast over the stack or not, as either operand."""
+    Z, R, C = shape
+    g = torch.Generator().manual_seed(1)
+    flat = torch.randn(Z * R * C + 16, generator=g).to(torch.float8_e4m3fn).to(DEV)
+    v = flat[start:start + Z * R * C].view(Z, R, C)
+    s = torch.ones(Z, 1 + (R - 1) // 128, 1 + (C - 1) // 128, device=DEV)
+    for values in (v, v[:1].expand(Z, R, C), v.mT):
+        sc = s if values.shape == v.shape else torch.ones(Z, 1 + (C - 1) // 128, 1 + (R - 1) // 128, device=DEV)
+        b = fp8.BlockTensor(values, sc)
+        dense = values.float()
+        other = fp8.quantize(torch.randint(-4, 5, (Z, 24, values.shape[1]), generator=g).float().to(DEV))
+        y = fp8.matmul(other, b, out_dtype=torch.float32)
+        ref.check(y, (other.dequantize() .double() @ dense.double()).cpu(), (other.dequantize().double().abs() @ dense.double().abs()).cpu(), R)
+        y = fp8.matmul(b, fp8.quantize(torch.ones(Z, values.shape[2], 3, device=DEV)), out_dtype=torch.float32)
+        ref.check(y, dense.double().cpu().sum(2, keepdim=True).expand(-1, -1, 3), dense.double().cpu().abs().sum(2, keepdim=True).expand(-1, -1, 3), C)
+
+
 def test_matmul_not_finite():
     """NaN reaches its row or column and nothing else; infinite and NaN elements behind the matrix's end are not read."""
     a, b = _rand((1, 130, 200), 1), _rand((1, 200, 140), 2)
