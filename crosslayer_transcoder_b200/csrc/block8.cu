@@ -56,6 +56,14 @@ struct Vec8Half {
     return m;
   }
   __device__ __forceinline__ void load(const T* p) { a = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  // from any address: the words that hold the values, two bytes more at either end where it is not a word's
+  __device__ __forceinline__ void load_words(const T* p) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
+    const int shift = ((uintptr_t)p & 2) * 8;
+    const uint32_t v[5] = {__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3), shift ? __ldg(w + 4) : 0u};
+    a = make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift), __funnelshift_r(v[2], v[3], shift),
+                   __funnelshift_r(v[3], v[4], shift));
+  }
   __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<uint4*>(p), a); }
 };
 template <>
@@ -107,6 +115,8 @@ __device__ __forceinline__ Vec8<T> load8(const T* p, int n, bool vec) {
   Vec8<T> r;
   if (vec) {
     r.load(p);
+  } else if (sizeof(T) == 2 && n >= 8) {
+    if constexpr (sizeof(T) == 2) r.load_words(p);
   } else {
     float v[8];
 #pragma unroll
@@ -359,6 +369,58 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
   for (int h = 0; h < 2; ++h) store8<T>(o + 8 * h, left - 8 * h, out_vec && left >= 8 * h + 8, f[h]);
 }
 
+// The same where the result's rows do not start on 16 bytes: 8 values to a thread, counted through all rows, so that every store but
+// the last is whole.  words: the copy's rows and their distances are multiples of 4 bytes.
+template <class T>
+__global__ void __launch_bounds__(256) dequantize_flat_kernel(const uint8_t* __restrict__ q, long long q_ld, long long q_z, ScaleMap sc,
+                                                              T* __restrict__ out, int R, unsigned C, long long n, int words) {
+  const long long i = (blockIdx.x * 256ll + threadIdx.x) * 8;
+  if (i >= n) return;
+  long long row = i / C;
+  unsigned c = (unsigned)(i - row * C);
+  long long z = row / R, r = row - z * R;
+  const uint8_t* p = q + z * q_z + r * q_ld + c;
+  const float* s = sc.p + z * sc.z + (r >> sc.shift) * sc.r;
+  float f[8];
+  if (c + 8 <= C) {
+    uint32_t w[2] = {0, 0};
+    if (words) {
+      const uint32_t* v = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
+      const int shift = ((uintptr_t)p & 3) * 8;
+      const uint32_t a = __ldg(v), b = __ldg(v + 1), d = shift ? __ldg(v + 2) : 0u;
+      w[0] = __funnelshift_r(a, b, shift), w[1] = __funnelshift_r(b, d, shift);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k >> 2] |= (uint32_t)p[k] << 8 * (k & 3);
+    }
+    const float s0 = __ldg(s + (c >> 7) * sc.c), s1 = __ldg(s + ((c + 7) >> 7) * sc.c);
+    const unsigned left = 128 - (c & 127);  // values of the first block
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t two = (w[k >> 1] >> 16 * (k & 1)) & 0xffff;
+      const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+      f[2 * k] = t.x * (2 * k < left ? s0 : s1), f[2 * k + 1] = t.y * (2 * k + 1 < left ? s0 : s1);
+    }
+  } else {  // into the next row
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      f[k] = 0.f;
+      if (i + k < n) {
+        const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)*p, __NV_E4M3);
+        f[k] = __half2float(__half(h)) * __ldg(s + (c >> 7) * sc.c);
+        ++p;
+        if (++c == C && i + k + 1 < n) {
+          c = 0;
+          if (++r == R) r = 0, ++z;
+          p = q + z * q_z + r * q_ld;
+          s = sc.p + z * sc.z + (r >> sc.shift) * sc.r;
+        }
+      }
+    }
+  }
+  store8<T>(out + i, (int)(n - i < 8 ? n - i : 8), n - i >= 8, f);
+}
+
 // Rows of bytes that start anywhere, to rows that start on 16 bytes: 16 of them to a thread, joined of five aligned words (bytes, at
 // the matrix's ends).
 __global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* __restrict__ q, long long q_ld, long long q_z,
@@ -413,12 +475,14 @@ constexpr int kRowsAhead = 4;
 struct Window {
   float lo[8], hi[8], theta[8];
 };
+// x > theta and x > 0; nothing is above a NaN
+__device__ __forceinline__ float threshold(float t) { return t != t ? __uint_as_float(0x7f800000u) : fmaxf(t, 0.f); }
 __device__ __forceinline__ void load_window(Window& w, const float* theta, Bandwidth bandwidth, int c, int n) {
   const double half = 0.5 * (double)bandwidth.get();
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     const float t = k < n ? theta[c + k] : 0.f;
-    w.theta[k] = t != t ? __uint_as_float(0x7f800000u) : fmaxf(t, 0.f);  // x > theta and x > 0; nothing is above a NaN
+    w.theta[k] = threshold(t);
     w.lo[k] = __double2float_rd((double)t - half);
     w.hi[k] = __double2float_rd((double)t + half);
   }
@@ -503,6 +567,78 @@ __global__ void __launch_bounds__(256) jump_relu_bwd_kernel(const T* __restrict_
   }
 }
 
+// The same where rows do not start on 16 bytes: a lane's 8 columns are 32 apart, so that a warp's accesses are side by side, and the
+// bits of 8 neighbours come from ballots.
+template <class T, bool kJump>
+__global__ void __launch_bounds__(256) jump_relu_fwd_strided_kernel(const T* __restrict__ x, long long ld,
+                                                                    const float* __restrict__ theta, Bandwidth bandwidth,
+                                                                    T* __restrict__ y, uint16_t* __restrict__ bits, int R, int C,
+                                                                    int rows_per_cta) {
+  const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 256, words = (C + 7) / 8;
+  if (c0 >= C) return;
+  float lo[8], hi[8], th[8];
+  if constexpr (kJump) {
+    const double half = 0.5 * (double)bandwidth.get();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = c0 + 32 * k + lane;
+      const float t = c < C ? theta[c] : 0.f;
+      th[k] = threshold(t);
+      lo[k] = __double2float_rd((double)t - half), hi[k] = __double2float_rd((double)t + half);
+    }
+  }
+  const int r1 = min(R, (int)(blockIdx.y + 1) * rows_per_cta), word = c0 / 8 + lane;
+#pragma unroll 2
+  for (int r = blockIdx.y * rows_per_cta; r < r1; ++r) {
+    const T* from = x + r * ld + c0 + lane;
+    T* to = y + (long long)r * C + c0 + lane;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c0 + 32 * k + lane < C ? to_f32(from[32 * k]) : 0.f;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float t = v[k];
+      const uint32_t pass = __ballot_sync(0xffffffffu, kJump ? !(t < 0.f) : !(t <= 0.f));
+      uint32_t in = 0;
+      if constexpr (kJump) in = __ballot_sync(0xffffffffu, t > lo[k] && t <= hi[k]);
+      if (lane >> 2 == k) mine = (pass >> 8 * (lane & 3) & 255) | (in >> 8 * (lane & 3) & 255) << 8;
+      if (c0 + 32 * k + lane < C) from_f32(to[32 * k], t <= (kJump ? th[k] : 0.f) ? 0.f : t);
+    }
+    if (word < words) bits[(long long)r * words + word] = (uint16_t)mine;
+  }
+}
+
+template <class T, bool kJump>
+__global__ void __launch_bounds__(256) jump_relu_bwd_strided_kernel(const T* __restrict__ g, long long ld,
+                                                                    const uint16_t* __restrict__ bits, T* __restrict__ dx,
+                                                                    float* __restrict__ part, int R, int C, int rows_per_cta) {
+  const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 256, words = (C + 7) / 8;
+  if (c0 >= C) return;
+  const int r1 = min(R, (int)(blockIdx.y + 1) * rows_per_cta), word = c0 / 8 + lane;
+  float acc[8] = {};
+#pragma unroll 2
+  for (int r = blockIdx.y * rows_per_cta; r < r1; ++r) {
+    const T* from = g + r * ld + c0 + lane;
+    T* to = dx + (long long)r * C + c0 + lane;
+    const uint32_t mine = word < words ? bits[(long long)r * words + word] : 0u;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = c0 + 32 * k + lane < C ? to_f32(from[32 * k]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t m = __shfl_sync(0xffffffffu, mine, 4 * k + (lane >> 3)) >> (lane & 7);
+      if (kJump && (m & 256)) acc[k] += v[k];
+      if (c0 + 32 * k + lane < C) from_f32(to[32 * k], m & 1 ? v[k] : 0.f);
+    }
+  }
+  if constexpr (kJump) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c0 + 32 * k + lane < C) part[(long long)blockIdx.y * C + c0 + 32 * k + lane] = acc[k];
+  }
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 long long up(long long a, long long b) { return (a + b - 1) / b; }
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
@@ -563,6 +699,14 @@ int quantize_any_list(const uint64_t* blocks, int n, int in_dtype, uint8_t* q, i
 
 template <class T>
 int dequantize(const uint8_t* q, long long q_ld, long long q_z, const ScaleMap& sc, T* out, int Z, int R, int C, cudaStream_t st) {
+  if (aligned16(out) && (long long)C * sizeof(T) % 16 != 0) {
+    const long long n = (long long)Z * R * C, grid = up(n, 2048);
+    CLT_CHECK_ARG(grid < (1ll << 31), "fp8_dequantize: too many values");
+    dequantize_flat_kernel<T><<<(unsigned)grid, 256, 0, st>>>(q, q_ld, q_z, sc, out, R, (unsigned)C, n,
+                                                              (uintptr_t)q % 4 == 0 && q_ld % 4 == 0 && q_z % 4 == 0);
+    CLT_CHECK_CUDA(cudaGetLastError());
+    return 0;
+  }
   const int groups = (int)up(C, 16);
   const long long n = (long long)Z * R * groups, grid = up(n, 256);
   CLT_CHECK_ARG(grid < (1ll << 31), "fp8_dequantize: too many values");
@@ -579,7 +723,12 @@ int jump_fwd(const T* x, long long ld, const float* theta, Bandwidth bw, T* y, u
   const int rows = rows_per_cta(R, C, sms);
   const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
   const int iv = aligned16(x) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(y) && C * (long long)sizeof(T) % 16 == 0;
-  if (theta != nullptr)
+  if (!iv || !ov) {
+    if (theta != nullptr)
+      jump_relu_fwd_strided_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
+    else
+      jump_relu_fwd_strided_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
+  } else if (theta != nullptr)
     jump_relu_fwd_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
   else
     jump_relu_fwd_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
@@ -593,9 +742,15 @@ int jump_bwd(const T* g, long long ld, const uint16_t* bits, const float* theta,
   const int rows = rows_per_cta(R, C, sms);
   const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
   const int iv = aligned16(g) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(dx) && C * (long long)sizeof(T) % 16 == 0;
+  const bool strided = !iv || !ov;
   if (theta != nullptr) {
-    jump_relu_bwd_kernel<T, true><<<grid, 256, 0, st>>>(g, ld, bits, dx, ws, R, C, rows, iv, ov);
+    if (strided)
+      jump_relu_bwd_strided_kernel<T, true><<<grid, 256, 0, st>>>(g, ld, bits, dx, ws, R, C, rows);
+    else
+      jump_relu_bwd_kernel<T, true><<<grid, 256, 0, st>>>(g, ld, bits, dx, ws, R, C, rows, iv, ov);
     sum_chunks_kernel<<<dim3((unsigned)up(C, 256), 1), 256, 0, st>>>(ws, dtheta, (int)grid.y, C, theta, bw);
+  } else if (strided) {
+    jump_relu_bwd_strided_kernel<T, false><<<grid, 256, 0, st>>>(g, ld, bits, dx, nullptr, R, C, rows);
   } else {
     jump_relu_bwd_kernel<T, false><<<grid, 256, 0, st>>>(g, ld, bits, dx, nullptr, R, C, rows, iv, ov);
   }
