@@ -587,25 +587,50 @@ __global__ void __launch_bounds__(256) jump_relu_fwd_strided_kernel(const T* __r
       lo[k] = __double2float_rd((double)t - half), hi[k] = __double2float_rd((double)t + half);
     }
   }
-  const int r1 = min(R, (int)(blockIdx.y + 1) * rows_per_cta), word = c0 / 8 + lane;
-#pragma unroll 2
-  for (int r = blockIdx.y * rows_per_cta; r < r1; ++r) {
-    const T* from = x + r * ld + c0 + lane;
-    T* to = y + (long long)r * C + c0 + lane;
-    float v[8];
+  const int r0 = blockIdx.y * rows_per_cta, n = min(R, r0 + rows_per_cta) - r0, left = C - c0 - lane;  // columns from this lane's on
+  const T* from = x + r0 * ld + c0 + lane;
+  T* to = y + (long long)r0 * C + c0 + lane;
+  uint16_t* word = bits + (long long)r0 * words + c0 / 8 + lane;
+  const bool whole = c0 + 256 <= C, has_word = c0 / 8 + lane < words;
+  for (int r = 0; r < n; r += 2) {
+    float v[2][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c0 + 32 * k + lane < C ? to_f32(from[32 * k]) : 0.f;
-    uint32_t mine = 0;
+    for (int i = 0; i < 2; ++i) {
+      const bool there = r + i < n;
+      if (whole && there) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float t = v[k];
-      const uint32_t pass = __ballot_sync(0xffffffffu, kJump ? !(t < 0.f) : !(t <= 0.f));
-      uint32_t in = 0;
-      if constexpr (kJump) in = __ballot_sync(0xffffffffu, t > lo[k] && t <= hi[k]);
-      if (lane >> 2 == k) mine = (pass >> 8 * (lane & 3) & 255) | (in >> 8 * (lane & 3) & 255) << 8;
-      if (c0 + 32 * k + lane < C) from_f32(to[32 * k], t <= (kJump ? th[k] : 0.f) ? 0.f : t);
+        for (int k = 0; k < 8; ++k) v[i][k] = to_f32(from[32 * k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = there && 32 * k < left ? to_f32(from[32 * k]) : 0.f;
+      }
+      from += ld;
     }
-    if (word < words) bits[(long long)r * words + word] = (uint16_t)mine;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (r + i < n) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float t = v[i][k];
+          const uint32_t pass = __ballot_sync(0xffffffffu, kJump ? !(t < 0.f) : !(t <= 0.f));
+          uint32_t in = 0;
+          if constexpr (kJump) in = __ballot_sync(0xffffffffu, t > lo[k] && t <= hi[k]);
+          if (lane >> 2 == k) mine = __byte_perm(pass >> 8 * (lane & 3), in >> 8 * (lane & 3), 0x0040);
+          v[i][k] = t <= (kJump ? th[k] : 0.f) ? 0.f : t;
+        }
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) from_f32(to[32 * k], v[i][k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (32 * k < left) from_f32(to[32 * k], v[i][k]);
+        }
+        if (has_word) *word = (uint16_t)mine;
+      }
+      to += C, word += words;
+    }
   }
 }
 
@@ -615,27 +640,53 @@ __global__ void __launch_bounds__(256) jump_relu_bwd_strided_kernel(const T* __r
                                                                     float* __restrict__ part, int R, int C, int rows_per_cta) {
   const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 256, words = (C + 7) / 8;
   if (c0 >= C) return;
-  const int r1 = min(R, (int)(blockIdx.y + 1) * rows_per_cta), word = c0 / 8 + lane;
+  const int r0 = blockIdx.y * rows_per_cta, n = min(R, r0 + rows_per_cta) - r0, left = C - c0 - lane;
+  const T* from = g + r0 * ld + c0 + lane;
+  T* to = dx + (long long)r0 * C + c0 + lane;
+  const uint16_t* word = bits + (long long)r0 * words + c0 / 8 + lane;
+  const bool whole = c0 + 256 <= C, has_word = c0 / 8 + lane < words;
   float acc[8] = {};
-#pragma unroll 2
-  for (int r = blockIdx.y * rows_per_cta; r < r1; ++r) {
-    const T* from = g + r * ld + c0 + lane;
-    T* to = dx + (long long)r * C + c0 + lane;
-    const uint32_t mine = word < words ? bits[(long long)r * words + word] : 0u;
-    float v[8];
+  for (int r = 0; r < n; r += 2) {
+    float v[2][8];
+    uint32_t mine[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c0 + 32 * k + lane < C ? to_f32(from[32 * k]) : 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const bool there = r + i < n;
+      mine[i] = there && has_word ? *word : 0u;
+      if (whole && there) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t m = __shfl_sync(0xffffffffu, mine, 4 * k + (lane >> 3)) >> (lane & 7);
-      if (kJump && (m & 256)) acc[k] += v[k];
-      if (c0 + 32 * k + lane < C) from_f32(to[32 * k], m & 1 ? v[k] : 0.f);
+        for (int k = 0; k < 8; ++k) v[i][k] = to_f32(from[32 * k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = there && 32 * k < left ? to_f32(from[32 * k]) : 0.f;
+      }
+      from += ld, word += words;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (r + i < n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t m = __shfl_sync(0xffffffffu, mine[i], 4 * k + (lane >> 3)) >> (lane & 7);
+          if (kJump && (m & 256)) acc[k] += v[i][k];
+          if (!(m & 1)) v[i][k] = 0.f;
+        }
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) from_f32(to[32 * k], v[i][k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (32 * k < left) from_f32(to[32 * k], v[i][k]);
+        }
+      }
+      to += C;
     }
   }
   if constexpr (kJump) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (c0 + 32 * k + lane < C) part[(long long)blockIdx.y * C + c0 + 32 * k + lane] = acc[k];
+      if (32 * k < left) part[(long long)blockIdx.y * C + c0 + 32 * k + lane] = acc[k];
   }
 }
 
