@@ -115,8 +115,15 @@ __device__ __forceinline__ Vec8<T> load8(const T* p, int n, bool vec) {
   Vec8<T> r;
   if (vec) {
     r.load(p);
-  } else if (sizeof(T) == 2 && n >= 8) {
-    if constexpr (sizeof(T) == 2) r.load_words(p);
+  } else if (n >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      r.load_words(p);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __ldg(p + i);
+      r.put(v);
+    }
   } else {
     float v[8];
 #pragma unroll
