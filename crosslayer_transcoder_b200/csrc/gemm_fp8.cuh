@@ -384,11 +384,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           const int kb1 = min(kb_per_seg, kb0 + left);
           left -= kb1 - kb0;
           for (int kb = kb0; kb < kb1; ++kb) {
-            if (!wait(empty0 + 8 * stage, phase ^ 1, abort_flag, status, kTimeoutEmpty)) {
-              alive = false;
-              break;
-            }
-            __syncwarp();
+            // (the vote: lanes that give up a wait at different times leave together)
+            alive = __all_sync(0xffffffffu, wait(empty0 + 8 * stage, phase ^ 1, abort_flag, status, kTimeoutEmpty));
+            if (!alive) break;
             if (one) {
               const uint32_t full = lead0 + 8 * stage;
               if (rank == 0) tc::mbar_expect_tx(full0 + 8 * stage, TL::kCtas * kStageBytes);
@@ -412,7 +410,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
           }
           kb0 = 0;
         }
-        alive = __all_sync(0xffffffffu, alive);
       }
       if constexpr (kPair) {
         // the leader's MMAs read this CTA's stages and its commits arrive here: stay until the last has
@@ -453,21 +450,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
             const int slot = batch % kSlots, in_window = min(left, window);
             uint32_t starts = 0xffffffffu;
             if constexpr (!kByRow) {
-              if (!wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutFull)) {
-                alive = false;
-                break;
-              }
+              alive = __all_sync(0xffffffffu, wait(tc::smem_u32(&ring->full[slot]), (batch / kSlots) & 1, abort_flag, status, kTimeoutFull));
+              if (!alive) break;
               starts = ring->starts[slot];
             }
             for (int i = 0; i < in_window; ++i) {
               const uint32_t buf = n & 1;
               const bool first = starts >> i & 1, last = i + 1 == in_window || (starts >> (i + 1) & 1);
-              if ((first && !wait(acc_empty0 + 8 * buf, ((n >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty)) ||
-                  !wait(full0 + 8 * stage, phase, abort_flag, status, kTimeoutFull)) {
-                alive = false;
-                break;
-              }
-              __syncwarp();
+              const bool ok = (!first || wait(acc_empty0 + 8 * buf, ((n >> 1) & 1) ^ 1, abort_flag, status, kTimeoutTmemEmpty)) &&
+                              wait(full0 + 8 * stage, phase, abort_flag, status, kTimeoutFull);
+              alive = __all_sync(0xffffffffu, ok);
+              if (!alive) break;
               tc::tc_fence_after();
               if (one) {
                 const uint32_t tmem_d = tmem_base + buf * kBN;
