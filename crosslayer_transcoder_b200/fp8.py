@@ -83,6 +83,14 @@ def _check(name: str, t, dtypes, device=None):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+MOST = 2 ** 31 - 256    # rows or columns of a matrix: the kernels count them, rounded up to tiles, in 32 bits
+
+
+def _fits(name: str, *sizes: int):
+    if max(sizes) > MOST:
+        raise ValueError(f"{name} has {' x '.join(map(str, sizes))} elements, at most {MOST} along an axis are supported")
+
+
 _checked = set()        # devices that the library runs on
 
 
@@ -133,6 +141,7 @@ class BlockTensor:
         want = (*shape[:-2], _blocks(shape[-2], block_rows), _blocks(shape[-1]))
         if scales.shape != want:
             raise ValueError(f"scales {tuple(scales.shape)} do not match {want}")
+        _fits("values", *shape)
         self.values, self.scales, self.block_rows, self.transposed = values, scales, block_rows, False
 
     @classmethod
@@ -156,7 +165,7 @@ class BlockTensor:
         return self._of(self.values, self.scales, self.block_rows, not self.transposed)
 
     def __getitem__(self, i: int) -> "BlockTensor":
-        if self.values.dim() != 3 or not isinstance(i, int):
+        if self.values.dim() != 3 or type(i) is not int:     # (True would add an axis)
             raise ValueError("a stack of matrices is indexed with one integer")
         return self._of(self.values[i], self.scales[i], self.block_rows, self.transposed)
 
@@ -207,6 +216,7 @@ def quantize(x: torch.Tensor, block_rows: int = BLOCK) -> BlockTensor:
         raise ValueError(f"expected a matrix or a stack of matrices, got {tuple(x.shape)}")
     if block_rows not in (1, BLOCK):
         raise ValueError(f"blocks of {block_rows} rows: 1 or 128 are supported")
+    _fits("x", *x.shape)
     return _on(x.device, _quantize_any, x.detach(), block_rows)
 
 
@@ -398,6 +408,8 @@ def project(x: torch.Tensor, W: torch.Tensor, b: Optional[torch.Tensor] = None) 
         _check("b", b, DTYPE_CODE, x.device)
         if b.shape != (ws[-1:] if one else (ws[0], ws[2])):
             raise ValueError(f"b {tuple(b.shape)} does not match W {tuple(ws)}")
+    _fits("x", xs.numel() // ws[:inner].numel(), ws[-2])
+    _fits("W", ws[-2], ws[-1])
     return _Project.apply(x, W, b)
 
 
@@ -455,6 +467,8 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
         _check("b", b, DTYPE_CODE, features.device)
         if b.shape != (L, D):
             raise ValueError(f"b {tuple(b.shape)} does not match {(L, D)}")
+    _fits("features", shape.numel() // (L * F), F)
+    _fits("blocks", F, D)
     return _CrosslayerDecode.apply(features, b, *blocks)
 
 
@@ -552,4 +566,5 @@ def jump_relu(x: torch.Tensor, theta: Optional[torch.Tensor] = None, bandwidth=1
                 raise ValueError(f"bandwidth has {bandwidth.numel()} elements")
         elif not float(bandwidth) > 0:
             raise ValueError(f"bandwidth must be positive, got {bandwidth}")
+    _fits("x", x.numel() // C if C else 0, C)
     return _JumpReLU.apply(x, theta, bandwidth, C)

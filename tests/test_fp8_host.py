@@ -178,3 +178,32 @@ def test_library_refuses():
             call("clt_fp8_pass_bwd", *bad)
     with pytest.raises(CltError, match="bad dims"):
         call("clt_sum_chunks", p, p, 0, 1, 8, None)
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 255, 2 ** 31, 2 ** 32 + 5])
+def test_axes_beyond_32_bits_are_refused(n):
+    """The library's sizes are C ints: a larger one would arrive as another number."""
+    W, decoder = _meta(1, 1, 8), [_meta(1, 1, 8)]
+    for call in (lambda: fp8.quantize(_meta(n, 1)), lambda: fp8.quantize(_meta(2, n)), lambda: fp8.quantize(_meta(n, 1, 1)),
+                 lambda: fp8.BlockTensor(_meta(n, 1, dtype=torch.float8_e4m3fn), _meta(n, 1, dtype=torch.float32), 1),
+                 lambda: fp8.project(_meta(n, 1, 1), W), lambda: fp8.project(_meta(n // 2 + 1, 2, 1, 1), W),
+                 lambda: fp8.project(_meta(4, 1), _meta(1, n)), lambda: fp8.crosslayer_decode(_meta(n, 1, 1), decoder),
+                 lambda: fp8.crosslayer_decode(_meta(4, 1, n), [_meta(1, n, 2)]),
+                 lambda: fp8.jump_relu(_meta(n)), lambda: fp8.jump_relu(_meta(n, 1), _meta(1))):
+        with pytest.raises(ValueError, match="at most"):
+            call()
+
+
+def test_largest_axis_is_taken():
+    with pytest.raises(CltError, match="CUDA tensors only"):
+        fp8.quantize(_meta(fp8.MOST, 1))
+
+
+def test_a_stack_is_indexed_with_integers_alone():
+    with pytest.raises(ValueError):
+        _block(Z=2)[True]
+    assert _block(Z=2)[-1].shape == (256, 256)
