@@ -7,7 +7,7 @@
 // infinity: what is not finite becomes NaN, and does not count for the scale.
 //
 // All kernels here are bound by memory: 12 x 4000 x 10000 bf16 to 8 bits 231 us (6.2 TB/s), back 226 (6.4); a gradient with its column
-// sums, 12 x 4000 x 24576, 573 (6.2); (Jump)ReLU of that size 856 (5.9) and its backward 806 (6.2).
+// sums, 12 x 4000 x 24576, 573 (6.2); JumpReLU of that size 780 (6.4) and its backward 790 (6.3), ReLU 765 (6.5) and 723 (6.9).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -488,64 +488,142 @@ __global__ void __launch_bounds__(256) sum_chunks_kernel(const float* __restrict
 }
 
 // ---- (Jump)ReLU with a two-bit checkpoint ---------------------------------------------------------------
-// A thread has 8 columns with their thresholds and walks down the rows, kRowsAhead of them in flight.  A word of the checkpoint is 16 bits for 8
-// values: the low byte has bit i where the gradient passes (x >= 0; ReLU: x > 0), the high byte where theta - bw/2 < x <= theta + bw/2,
-// the window in which the threshold gets a gradient.  Both bounds are rounded down from 64 bits, which decides the comparisons with
-// an fp32 x as the exact bounds would.
+// A thread has 8 columns and kRowsAhead rows of them in flight.  A word of the checkpoint is 16 bits for 8 values: the low byte has
+// bit i where the gradient passes (x >= 0; ReLU: x > 0), the high byte where theta - bw/2 < x <= theta + bw/2, the window in which the
+// threshold gets a gradient.  Both bounds are rounded down, once, which decides the comparisons with an fp32 x as the exact bounds
+// would.
 constexpr int kRowsAhead = 4;
+// the row behind the CTA's last
+__device__ __forceinline__ int row_end(int R, int rows) { return (int)min((long long)R, (blockIdx.y + 1ll) * rows); }
 struct Window {
   float lo[8], hi[8], theta[8];
+};
+// 16-bit values are compared two at a time with the bounds in their own type, rounded down once more (820 -> 785 us, 16 rows to a
+// thread).
+template <class T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ type down(float a, float b) { return __halves2half2(__float2half_rd(a), __float2half_rd(b)); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ type down(float a, float b) { return __halves2bfloat162(__float2bfloat16_rd(a), __float2bfloat16_rd(b)); }
+};
+template <class T>
+struct PackedWindow {
+  using P = typename Pair<T>::type;
+  P lo[4], hi[4], theta[4];
+  __device__ __forceinline__ explicit PackedWindow(const Window& w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lo[i] = Pair<T>::down(w.lo[2 * i], w.lo[2 * i + 1]), hi[i] = Pair<T>::down(w.hi[2 * i], w.hi[2 * i + 1]);
+      theta[i] = Pair<T>::down(w.theta[2 * i], w.theta[2 * i + 1]);
+    }
+  }
+  // what is not above its threshold becomes 0; the word of the checkpoint
+  __device__ __forceinline__ uint32_t apply(uint4& v) const {
+    uint32_t x[4] = {v.x, v.y, v.z, v.w}, negative = 0, inside = 0;
+    const P zero = Pair<T>::down(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const P p = *reinterpret_cast<const P*>(&x[i]);
+      const uint32_t two = 1u << 2 * i | 2u << (2 * i + 16);  // bits 2i and 2i + 1 of the byte, the second in the upper half
+      negative |= __hlt2_mask(p, zero) & two;
+      inside |= __hgt2_mask(p, lo[i]) & __hle2_mask(p, hi[i]) & two;
+      x[i] &= ~__hle2_mask(p, theta[i]);
+    }
+    v = make_uint4(x[0], x[1], x[2], x[3]);
+    return (~(negative | negative >> 16) & 0xffu) | ((inside | inside >> 16) & 0xffu) << 8;
+  }
 };
 // x > theta and x > 0; nothing is above a NaN
 __device__ __forceinline__ float threshold(float t) { return t != t ? __uint_as_float(0x7f800000u) : fmaxf(t, 0.f); }
 __device__ __forceinline__ void load_window(Window& w, const float* theta, Bandwidth bandwidth, int c, int n) {
-  const double half = 0.5 * (double)bandwidth.get();
+  const float bw = bandwidth.get();
+  float t[8];
+  if (n >= 8 && ((uintptr_t)(theta + c) & 15) == 0) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(theta + c)), b = __ldg(reinterpret_cast<const float4*>(theta + c) + 1);
+    t[0] = a.x, t[1] = a.y, t[2] = a.z, t[3] = a.w, t[4] = b.x, t[5] = b.y, t[6] = b.z, t[7] = b.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[k] = k < n ? __ldg(theta + c + k) : 0.f;
+  }
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float t = k < n ? theta[c + k] : 0.f;
-    w.theta[k] = threshold(t);
-    w.lo[k] = __double2float_rd((double)t - half);
-    w.hi[k] = __double2float_rd((double)t + half);
+    w.theta[k] = threshold(t[k]);
+    w.lo[k] = __fmaf_rd(-0.5f, bw, t[k]), w.hi[k] = __fmaf_rd(0.5f, bw, t[k]);
   }
 }
+
+// The sums of a CTA's 8 warps over their rows, by column, in the warps' order.
+struct WarpSums {
+  float of[8][256];
+  __device__ __forceinline__ void out(float* part, int c0, int C) const {
+    __syncthreads();
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += of[i][threadIdx.x];
+    if (c0 + (int)threadIdx.x < C) part[(long long)blockIdx.y * C + c0 + threadIdx.x] = sum;
+  }
+};
 
 template <class T, bool kJump>
 __global__ void __launch_bounds__(256) jump_relu_fwd_kernel(const T* __restrict__ x, long long ld, const float* __restrict__ theta,
                                                             Bandwidth bandwidth, T* __restrict__ y, uint16_t* __restrict__ bits,
-                                                            int R, int C, int rows_per_cta, int in_vec, int out_vec) {
+                                                            int R, int C, int rows_per_cta) {
   const int words = (C + 7) / 8, w = blockIdx.x * 256 + threadIdx.x;
   if (w >= words) return;
-  const int c = w * 8, n = C - c;
-  Window win;
-  if constexpr (kJump) load_window(win, theta, bandwidth, c, n);
-  const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
-  const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
-  for (int r = r0; r < r1; r += kRowsAhead) {
-    Vec8<T> v[kRowsAhead];
+  const int c = w * 8, n = C - c;  // (fp32: the last 8 may be 4)
+  const int r0 = blockIdx.y * rows_per_cta, r1 = row_end(R, rows_per_cta);
+  Vec8<T> v[kRowsAhead];
+  const auto load = [&](int r) {
 #pragma unroll
-    for (int i = 0; i < kRowsAhead; ++i) v[i] = load8<T>(x + (r + i) * ld + c, r + i < r1 ? n : 0, iv && r + i < r1);
+    for (int i = 0; i < kRowsAhead; ++i) v[i] = load8<T>(x + (r + i) * ld + c, r + i < r1 ? n : 0, n >= 8 && r + i < r1);
+  };
+  load(r0);
+  const auto rows = [&](auto&& apply) {
+    for (int r = r0;;) {
 #pragma unroll
-    for (int i = 0; i < kRowsAhead; ++i) {
-      if (r + i < r1) {
-        float f[8];
-        v[i].get(f);
-        uint32_t m = 0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float t = f[k];
-          if constexpr (kJump) {
-            if (!(t < 0.f)) m |= 1u << k;
-            if (t > win.lo[k] && t <= win.hi[k]) m |= 256u << k;
-            f[k] = t <= win.theta[k] ? 0.f : t;  // (at least 0; NaN stays)
-          } else {
-            if (!(t <= 0.f)) m |= 1u << k;
-            f[k] = t <= 0.f ? 0.f : t;
-          }
-        }
-        store8<T>(y + (long long)(r + i) * C + c, n, ov, f);
-        bits[(long long)(r + i) * words + w] = (uint16_t)m;
-      }
+      for (int i = 0; i < kRowsAhead; ++i)
+        if (r + i < r1) bits[(long long)(r + i) * words + w] = (uint16_t)apply(v[i], y + (long long)(r + i) * C + c);
+      if ((r += kRowsAhead) >= r1) break;
+      load(r);
     }
+  };
+  if constexpr (kJump && sizeof(T) == 2) {
+    Window wide;  // (on its way with the first rows)
+    load_window(wide, theta, bandwidth, c, n);
+    const PackedWindow<T> win(wide);
+    rows([&](Vec8<T>& u, T* to) {
+      const uint32_t m = win.apply(u.a);
+      u.store(to);
+      return m;
+    });
+  } else {
+    Window win;
+    if constexpr (kJump) load_window(win, theta, bandwidth, c, n);
+    rows([&](Vec8<T>& u, T* to) {
+      float f[8];
+      u.get(f);
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float t = f[k];
+        if constexpr (kJump) {
+          if (!(t < 0.f)) m |= 1u << k;
+          if (t > win.lo[k] && t <= win.hi[k]) m |= 256u << k;
+          f[k] = t <= win.theta[k] ? 0.f : t;  // (at least 0; NaN stays)
+        } else {
+          if (!(t <= 0.f)) m |= 1u << k;
+          f[k] = t <= 0.f ? 0.f : t;
+        }
+      }
+      store8<T>(to, n, n >= 8, f);
+      return m;
+    });
   }
 }
 
@@ -553,13 +631,17 @@ template <class T, bool kJump>
 __global__ void __launch_bounds__(256) jump_relu_bwd_kernel(const T* __restrict__ g, long long ld, const uint16_t* __restrict__ bits,
                                                             T* __restrict__ dx, float* __restrict__ part, int R, int C,
                                                             int rows_per_cta, int in_vec, int out_vec) {
-  const int words = (C + 7) / 8, w = blockIdx.x * 256 + threadIdx.x;
-  if (w >= words) return;
+  // with a threshold's gradient a warp has 256 columns and the CTA's warps take rows in turn: its sums are made of many rows
+  // while a thread walks few of them
+  const int words = (C + 7) / 8, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = kJump ? blockIdx.x * 32 + lane : blockIdx.x * 256 + threadIdx.x;
+  if (!kJump && w >= words) return;
   const int c = w * 8, n = C - c;
-  const int r0 = blockIdx.y * rows_per_cta, r1 = min(R, r0 + rows_per_cta);
+  const int r1 = w < words ? row_end(R, rows_per_cta) : 0;
+  const int r0 = blockIdx.y * rows_per_cta + (kJump ? warp * kRowsAhead : 0), step = (kJump ? 8 : 1) * kRowsAhead;
   const bool iv = in_vec && n >= 8, ov = out_vec && n >= 8;
   float acc[8] = {};
-  for (int r = r0; r < r1; r += kRowsAhead) {
+  for (int r = r0; r < r1; r += step) {
     Vec8<T> v[kRowsAhead];
     uint32_t m[kRowsAhead];
 #pragma unroll
@@ -582,9 +664,11 @@ __global__ void __launch_bounds__(256) jump_relu_bwd_kernel(const T* __restrict_
     }
   }
   if constexpr (kJump) {
+    __shared__ WarpSums sums;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) part[(long long)blockIdx.y * C + c + k] = acc[k];
+    for (int k = 0; k < 8; k += 4)
+      *reinterpret_cast<float4*>(&sums.of[warp][lane * 8 + k]) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+    sums.out(part, blockIdx.x * 256, C);
   }
 }
 
@@ -599,17 +683,17 @@ __global__ void __launch_bounds__(256) jump_relu_fwd_strided_kernel(const T* __r
   if (c0 >= C) return;
   float lo[8], hi[8], th[8];
   if constexpr (kJump) {
-    const double half = 0.5 * (double)bandwidth.get();
+    const float bw = bandwidth.get();
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int c = c0 + 32 * k + lane;
-      const float t = c < C ? theta[c] : 0.f;
+      const float t = c < C ? __ldg(theta + c) : 0.f;
       th[k] = threshold(t);
-      lo[k] = __double2float_rd((double)t - half), hi[k] = __double2float_rd((double)t + half);
+      lo[k] = __fmaf_rd(-0.5f, bw, t), hi[k] = __fmaf_rd(0.5f, bw, t);
     }
   }
-  const int r0 = blockIdx.y * rows_per_cta, n = min(R, r0 + rows_per_cta) - r0, left = C - c0 - lane;  // columns from this lane's on
-  const T* from = x + r0 * ld + c0 + lane;
+  const int r0 = blockIdx.y * rows_per_cta, n = row_end(R, rows_per_cta) - r0, left = C - c0 - lane;  // columns from this lane's on
+  const T* from = x + (long long)r0 * ld + c0 + lane;
   T* to = y + (long long)r0 * C + c0 + lane;
   uint16_t* word = bits + (long long)r0 * words + c0 / 8 + lane;
   const bool whole = c0 + 256 <= C, has_word = c0 / 8 + lane < words;
@@ -659,15 +743,17 @@ template <class T, bool kJump>
 __global__ void __launch_bounds__(256) jump_relu_bwd_strided_kernel(const T* __restrict__ g, long long ld,
                                                                     const uint16_t* __restrict__ bits, T* __restrict__ dx,
                                                                     float* __restrict__ part, int R, int C, int rows_per_cta) {
-  const int lane = threadIdx.x & 31, c0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * 256, words = (C + 7) / 8;
-  if (c0 >= C) return;
-  const int r0 = blockIdx.y * rows_per_cta, n = min(R, r0 + rows_per_cta) - r0, left = C - c0 - lane;
-  const T* from = g + r0 * ld + c0 + lane;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = (kJump ? blockIdx.x : blockIdx.x * 8 + warp) * 256, words = (C + 7) / 8;
+  if (!kJump && c0 >= C) return;
+  // (with a threshold's gradient the warps take rows in turn, as above)
+  const int r0 = blockIdx.y * rows_per_cta + (kJump ? 2 * warp : 0), step = kJump ? 16 : 2, left = C - c0 - lane;
+  const int n = row_end(R, rows_per_cta) - r0;
+  const T* from = g + (long long)r0 * ld + c0 + lane;
   T* to = dx + (long long)r0 * C + c0 + lane;
   const uint16_t* word = bits + (long long)r0 * words + c0 / 8 + lane;
   const bool whole = c0 + 256 <= C, has_word = c0 / 8 + lane < words;
   float acc[8] = {};
-  for (int r = 0; r < n; r += 2) {
+  for (int r = 0; r < n; r += step) {
     float v[2][8];
     uint32_t mine[2];
 #pragma unroll
@@ -703,11 +789,13 @@ __global__ void __launch_bounds__(256) jump_relu_bwd_strided_kernel(const T* __r
       }
       to += C;
     }
+    if constexpr (kJump) from += (step - 2) * ld, word += (step - 2) * words, to += (long long)(step - 2) * C;
   }
   if constexpr (kJump) {
+    __shared__ WarpSums sums;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (32 * k < left) part[(long long)blockIdx.y * C + c0 + 32 * k + lane] = acc[k];
+    for (int k = 0; k < 8; ++k) sums.of[warp][32 * k + lane] = acc[k];
+    sums.out(part, c0, C);
   }
 }
 
@@ -715,13 +803,16 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 long long up(long long a, long long b) { return (a + b - 1) / b; }
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
-// Rows that one CTA of the (Jump)ReLU kernels walks: enough CTAs for the chip, at least 8 rows (a thread's thresholds are read once).
-int rows_per_cta(int R, int C, int sms) {
-  const long long across = up(up(C, 8), 256), want = up(8ll * sms, across);
-  long long rows = up(R, want), least = up(R, 65535);  // (a grid's y)
-  rows = rows < 8 ? 8 : rows > 128 ? 128 : rows;
-  return (int)(rows < least ? least : rows);
+// Rows of a CTA of the (Jump)ReLU kernels that has one of `across` pieces of them: enough CTAs for the chip, within bounds.  Few
+// rows, all of them in flight at once, are faster than a walk: 12 x 4000 x 24576 bf16 ReLU in 4 rows 765 us, in 128 848, and 6 x
+// 4000 x 10000 fp32 JumpReLU 293 and 336.  Where a thread's thresholds cost more than that: 8 rows for 16-bit values (780; 4: 863),
+// 64 for rows that are not aligned.  Where each CTA's sums go to memory and back, 32 to 128, which its 8 warps share.
+int rows_per_cta(int R, long long across, int least, int most, int sms) {
+  const long long rows = up(R, up(8ll * sms, across)), grid_y = up(R, 65535);
+  const long long bounded = rows < least ? least : rows > most ? most : rows;
+  return (int)(bounded < grid_y ? grid_y : bounded);
 }
+int rows_per_sum(int R, int C, int sms) { return rows_per_cta(R, up(C, 256), 32, 128, sms); }
 
 template <class T>
 int quantize(const Source& s, uint8_t* q, int q_ld, float* scales, float* sums, int Z, int block_rows, cudaStream_t st) {
@@ -792,18 +883,19 @@ int dequantize(const uint8_t* q, long long q_ld, long long q_z, const ScaleMap& 
 template <class T>
 int jump_fwd(const T* x, long long ld, const float* theta, Bandwidth bw, T* y, uint16_t* bits, int R, int C, int sms,
              cudaStream_t st) {
-  const int rows = rows_per_cta(R, C, sms);
-  const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
-  const int iv = aligned16(x) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(y) && C * (long long)sizeof(T) % 16 == 0;
-  if (!iv || !ov) {
+  const bool strided = !aligned16(x) || ld * (long long)sizeof(T) % 16 || !aligned16(y) || C * (long long)sizeof(T) % 16;
+  const long long across = up(up(C, 8), 256);
+  const int rows = rows_per_cta(R, across, 4, theta == nullptr ? 4 : strided ? 64 : sizeof(T) == 2 ? 8 : 4, sms);
+  const dim3 grid((unsigned)across, (unsigned)up(R, rows));
+  if (strided) {
     if (theta != nullptr)
       jump_relu_fwd_strided_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
     else
       jump_relu_fwd_strided_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
   } else if (theta != nullptr)
-    jump_relu_fwd_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
+    jump_relu_fwd_kernel<T, true><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
   else
-    jump_relu_fwd_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows, iv, ov);
+    jump_relu_fwd_kernel<T, false><<<grid, 256, 0, st>>>(x, ld, theta, bw, y, bits, R, C, rows);
   CLT_CHECK_CUDA(cudaGetLastError());
   return 0;
 }
@@ -811,8 +903,9 @@ int jump_fwd(const T* x, long long ld, const float* theta, Bandwidth bw, T* y, u
 template <class T>
 int jump_bwd(const T* g, long long ld, const uint16_t* bits, const float* theta, Bandwidth bw, T* dx, float* dtheta, float* ws,
              int R, int C, int sms, cudaStream_t st) {
-  const int rows = rows_per_cta(R, C, sms);
-  const dim3 grid((unsigned)up(up(C, 8), 256), (unsigned)up(R, rows));
+  const long long across = theta != nullptr ? up(C, 256) : up(up(C, 8), 256);
+  const int rows = theta != nullptr ? rows_per_sum(R, C, sms) : rows_per_cta(R, across, 4, 4, sms);
+  const dim3 grid((unsigned)across, (unsigned)up(R, rows));
   const int iv = aligned16(g) && ld * (long long)sizeof(T) % 16 == 0, ov = aligned16(dx) && C * (long long)sizeof(T) % 16 == 0;
   const bool strided = !iv || !ov;
   if (theta != nullptr) {
@@ -901,7 +994,7 @@ int clt_sum_chunks(const float* part, float* out, int Z, int chunks, int C, clt_
   return 0;
 }
 
-int clt_jump_relu_chunks(int R, int C) { return R > 0 && C > 0 ? (int)up(R, rows_per_cta(R, C, device_sm_count())) : 0; }
+int clt_jump_relu_chunks(int R, int C) { return R > 0 && C > 0 ? (int)up(R, rows_per_sum(R, C, device_sm_count())) : 0; }
 
 int clt_jump_relu_fwd(const void* x, int64_t ld, const float* theta, const float* bandwidth, float bandwidth_value, void* y,
                       void* bits, int dtype, int R, int C, clt_stream_t stream) {
@@ -911,7 +1004,6 @@ int clt_jump_relu_fwd(const void* x, int64_t ld, const float* theta, const float
   CLT_CHECK_ARG(dtype >= 0 && dtype <= 2 && (uintptr_t)x % elem_size(dtype) == 0 && (uintptr_t)y % elem_size(dtype) == 0,
                 "jump_relu_fwd: type %d or misaligned pointer", dtype);
   const int sms = device_sm_count();
-  CLT_CHECK_ARG(up(R, rows_per_cta(R, C, sms)) <= 65535, "jump_relu_fwd: too many rows");
   cudaStream_t st = (cudaStream_t)stream;
   uint16_t* b = (uint16_t*)bits;
   const Bandwidth bw{bandwidth, bandwidth_value};
@@ -929,8 +1021,7 @@ int clt_jump_relu_bwd(const void* g, int64_t ld, const void* bits, const float* 
   CLT_CHECK_ARG(dtype >= 0 && dtype <= 2 && (uintptr_t)g % elem_size(dtype) == 0 && (uintptr_t)dx % elem_size(dtype) == 0,
                 "jump_relu_bwd: type %d or misaligned pointer", dtype);
   const int sms = device_sm_count();
-  const long long chunks = up(R, rows_per_cta(R, C, sms));
-  CLT_CHECK_ARG(chunks <= 65535, "jump_relu_bwd: too many rows");
+  const long long chunks = up(R, rows_per_sum(R, C, sms));
   CLT_CHECK_ARG(theta == nullptr || chunks * C <= ws_floats, "jump_relu_bwd: %lld floats of scratch, %lld needed",
                 (long long)ws_floats, chunks * C);
   cudaStream_t st = (cudaStream_t)stream;

@@ -377,6 +377,53 @@ def test_jump_relu_special_values():
     assert torch.equal(torch.relu(x).isnan(), fp8.jump_relu(eager).isnan())
 
 
+def _inside(x, theta, half):
+    """theta - half < x <= theta + half exactly, in 64 bits: the rounded difference decides wherever it is not the half width itself
+    (rounding keeps the order), its error (Knuth's two-sum) where it is: -0.5 + 0.5 < 1e-40, though 1e-40 + 0.5 rounds to 0.5."""
+    d = x - theta
+    t = d - x
+    e = (x - (d - t)) + (-theta - t)
+    return ((d > -half) | (d == -half) & (e > 0)) & ((d < half) | (d == half) & (e <= 0))
+
+
+@pytest.mark.parametrize("as_fp32", [False, True])
+@pytest.mark.parametrize("columns", [16, 15])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_jump_relu_every_16_bit_value(dtype, columns, as_fp32):
+    """All 65536 values at thresholds and bandwidths up to the types' ends, aligned rows and others: results and checkpoint are
+    those of the exact comparisons."""
+    inf = float("inf")
+    x = torch.arange(-32768, 32768).to(torch.int16).view(dtype)[:, None].expand(65536, columns).contiguous().to(DEV)
+    if as_fp32:
+        x = x.float()
+    theta = torch.tensor([0.0, -0.5, 1e-3, 0.03, 65504.0, 1e6, -1e6, inf, float("nan"), 3.4e38, 1e-40, 2.0 ** -24, 0.53, -inf, 6e-8,
+                          1.0][:columns], device=DEV)
+    for bw in (1.0, 1e-6, 1e30, 1e-40, 2.0 ** -149):
+        y, bits = fp8._jump_relu_forward(x, columns, theta, None, bw)
+        bw = float(torch.tensor(bw))
+        xd, td = x.double(), theta.double()
+        want = torch.where((xd > td) & (xd > 0) | xd.isnan(), xd, torch.zeros_like(xd))
+        assert torch.equal(y.double().nan_to_num(nan=-9.0), want.nan_to_num(nan=-9.0))
+        words = bits.int() & 0xffff
+        at = torch.arange(columns, device=DEV)
+        word = words[:, at // 8]
+        assert torch.equal((word >> at % 8 & 1).bool(), ~(xd < 0))
+        assert torch.equal((word >> (8 + at % 8) & 1).bool(), _inside(xd, td, bw / 2))
+    fp8.check_status()
+
+
+@pytest.mark.parametrize("rows, columns", [(1, 24), (31, 520), (33, 2056), (129, 72), (1000, 264), (4100, 40), (515, 777)])
+def test_threshold_gradient_over_the_warps_rows(rows, columns):
+    """A CTA's warps share its rows: each row counts once, in the checkpoint's window, whatever the rows behind the last CTA's end."""
+    for dtype in TYPES:
+        x = torch.zeros(rows, columns, dtype=dtype, device=DEV).requires_grad_()
+        theta = torch.ones(columns, device=DEV, requires_grad=True)
+        g = (torch.arange(rows, device=DEV) % 7 + 1).to(dtype)[:, None].expand(rows, columns)
+        dx, dth = torch.autograd.grad(fp8.jump_relu(x, theta, 4.0), (x, theta), g)
+        assert torch.equal(dx, g)                # x = 0 passes the gradient
+        assert torch.equal(dth, (-g.double().sum(0) / 4).float())    # whole numbers below 2^24: sums and a quarter are exact
+
+
 def test_jump_relu_against_the_module():
     """The same results as model.JumpReLU's own autograd function."""
     from crosslayer_transcoder_b200.model import JumpReLU
