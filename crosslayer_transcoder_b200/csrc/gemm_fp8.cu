@@ -185,14 +185,15 @@ int dispatch(const GemmGeom& g, const tc::TcOperand& a, const tc::TcOperand& b, 
   CLT_CHECK_ARG(false, "fp8_matmul: operand layout");
 }
 
-// The 8-bit copy [Z, R, C] of a pass's operand in one buffer: values, rows of a multiple of 16, then scales of 128 x 128 blocks.
+// The 8-bit copy [Z, R, C] of a pass's operand in one buffer: values, rows of a multiple of 32 (a memory sector), then scales of 128 x 128
+// blocks.
 struct Copy {
   uint8_t* q;
   float* s;
   int64_t ld, z, sr, sz;  // distances of rows and matrices of the values, of rows and matrices of the scales
   long long bytes;
   Copy(void* buf, long long Z, long long R, long long C) {
-    ld = up(C, 16) * 16, z = R * ld, sr = up(C, 128), sz = up(R, 128) * sr;
+    ld = up(C, 32) * 32, z = R * ld, sr = up(C, 128), sz = up(R, 128) * sr;
     q = (uint8_t*)buf;
     s = (float*)(q + Z * z);
     bytes = Z * (z + 4 * sz);

@@ -113,14 +113,16 @@ def _first_order(backward):
 
 
 def _pitch(C: int) -> int:
-    return (C + 15) & ~15
+    """Bytes from row to row of a copy.  16 are enough for the contraction; rows that start on a memory sector are written faster
+    (12 x 4000 x 10000 bf16: 244 -> 225 us)."""
+    return (C + 31) & ~31
 
 
 def _storage(*shape, device):
-    """8-bit values [..., C] whose rows start on 16 bytes."""
+    """8-bit values [..., C] whose rows start on 32 bytes."""
     C = shape[-1]
     v = torch.empty(*shape[:-1], _pitch(C), dtype=torch.float8_e4m3fn, device=device)
-    return v if C % 16 == 0 else v[..., :C]
+    return v if C % 32 == 0 else v[..., :C]
 
 
 class BlockTensor:

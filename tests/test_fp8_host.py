@@ -104,8 +104,8 @@ def test_parts_cover_the_contraction(mode, M, N, K, L):
 
 @pytest.mark.parametrize("Z, R, C", [(1, 1, 1), (3, 136, 64), (12, 4000, 10000), (2, 129, 257)])
 def test_copies_have_room(Z, R, C):
-    """A copy's buffer holds its values, rows of a multiple of 16, and the scales of its blocks, and not 256 bytes more."""
-    need = Z * R * (-(-C // 16) * 16) + 4 * Z * -(-R // 128) * -(-C // 128)
+    """A copy's buffer holds its values, rows of a multiple of 32, and the scales of its blocks, and not 256 bytes more."""
+    need = Z * R * (-(-C // 32) * 32) + 4 * Z * -(-R // 128) * -(-C // 128)
     units = lib().query("clt_fp8_copy_units", Z, R, C)
     assert need <= 256 * units < need + 256
     assert lib().query("clt_fp8_copy_units", Z, 0, C) == 0
