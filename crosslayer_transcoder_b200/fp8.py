@@ -445,7 +445,10 @@ class _CrosslayerDecode(torch.autograd.Function):
         df, dW, db = _on(g.device, _pass_backward, 1, g.reshape(B, L, D), f_copy, w_copy, F, f_type, same, need_f, any(need_w), need_b)
         if db is not None and b_type != torch.float32:
             db = db.to(b_type)
-        parts = [dW[_pairs(t):_pairs(t + 1)].to(w_types[t]) if need else None for t, need in enumerate(need_w)]
+        parts = [None] * L
+        if dW is not None:
+            parts = [(p if dt == same else p.to(dt)) if need else None
+                     for p, dt, need in zip(dW.split(list(range(1, L + 1))), w_types, need_w)]
         return (None if df is None else df.view(ctx.shape), db, *parts)
 
 
@@ -462,9 +465,10 @@ def crosslayer_decode(features: torch.Tensor, blocks: Sequence[torch.Tensor], b:
         raise ValueError(f"{L} layers: at most 361 are supported")
     for t, w in enumerate(blocks):
         _check(f"blocks[{t}]", w, DTYPE_CODE, features.device)
-        if w.shape != (t + 1, F, blocks[0].shape[-1]) or w.numel() == 0:
-            raise ValueError(f"blocks[{t}] {tuple(w.shape)} does not match {(t + 1, F, blocks[0].shape[-1])}")
-    D = blocks[0].shape[2]
+    D = blocks[0].shape[-1] if blocks[0].dim() else 0
+    for t, w in enumerate(blocks):
+        if w.shape != (t + 1, F, D) or F * D == 0:
+            raise ValueError(f"blocks[{t}] {tuple(w.shape)} does not match {(t + 1, F, D)}, not empty")
     if b is not None:
         _check("b", b, DTYPE_CODE, features.device)
         if b.shape != (L, D):

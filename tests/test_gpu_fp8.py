@@ -326,6 +326,22 @@ def test_crosslayer_decode_block_forms():
     fp8.check_status()
 
 
+@pytest.mark.parametrize("needs", ["f", "b", "blocks", "one block", "f and b"])
+def test_crosslayer_decode_gradients_of_some(needs):
+    """What needs no gradient gets none, and the others' are the same bits as when all are asked for."""
+    L, F, D = 3, 40, 24
+    f, b = _rand((50, L, F), 1), _rand((L, D), 2)
+    blocks = [_rand((t + 1, F, D), 3 + t) for t in range(L)]
+    g = _rand((50, L, D), 9)
+    every = [x.clone().requires_grad_() for x in (f, b, *blocks)]
+    want = torch.autograd.grad(fp8.crosslayer_decode(every[0], every[2:], every[1]), every, g)
+    at = {"f": [0], "b": [1], "blocks": [2, 3, 4], "one block": [3], "f and b": [0, 1]}[needs]
+    some = [x.clone().requires_grad_(i in at) for i, x in enumerate((f, b, *blocks))]
+    fp8.crosslayer_decode(some[0], some[2:], some[1]).backward(g)
+    for i, x in enumerate(some):
+        assert torch.equal(x.grad, want[i]) if i in at else x.grad is None
+
+
 # ---- (Jump)ReLU ----------------------------------------------------------------------------------------------------------------
 def _jump_reference(x, theta, bw, g):
     x, g, th = x.double().cpu(), g.double().cpu(), theta.double().cpu()
