@@ -209,8 +209,12 @@ class CrossLayerTranscoder(SerializableModule):
 
     def _forward_eight_bit(self, acts):
         """The three products of ``forward`` through ``crosslayer_transcoder_b200.fp8``, results in the type of ``acts``.  Nonlinearities
-        other than (Jump)ReLU are the module's own."""
+        other than (Jump)ReLU are the module's own.  A feature shard (``parallel.attach``) is refused: its features give a part of
+        the sum over all shards, and a TopK would select within the shard."""
         enc, dec, nl = self.encoder, self.decoder, self.nonlinearity
+        engine = enc.__dict__.get("_kernel_engine")
+        if engine is not None and getattr(engine.module, "tp_world", 1) > 1:
+            raise NotImplementedError("eight_bit runs on whole modules only, not on feature shards")
         pre_actvs = fp8.project(acts, enc.W, enc.b)
         if isinstance(nl, JumpReLU):
             features = fp8.jump_relu(pre_actvs, nl.theta, nl.bandwidth)

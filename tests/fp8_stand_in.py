@@ -1,0 +1,28 @@
+"""The passes of the 8-bit operators in plain torch, for tests of the code around them that run on the CPU."""
+import torch
+
+from crosslayer_transcoder_b200 import fp8
+
+
+def project(x, W, b=None):
+    y = torch.einsum("...ld,ldf->...lf", x, W)
+    return y if b is None else y + b
+
+
+def crosslayer_decode(features, blocks, b=None):
+    y = torch.stack([torch.einsum("bsf,sfd->bd", features[:, :t + 1], w) for t, w in enumerate(blocks)], 1)
+    return y if b is None else y + b
+
+
+def jump_relu(x, theta=None, bandwidth=1.0):
+    """Which thresholds the operator takes is part of what is tested: they have the shape of x's last axes."""
+    if theta is None:
+        return torch.relu(x)
+    inner = theta.shape[1:] if theta.shape[0] == 1 else theta.shape
+    assert x.shape[x.dim() - len(inner):] == inner
+    return x * ((x > theta) & (x > 0))
+
+
+def install(setattr_=setattr):
+    for f in (project, crosslayer_decode, jump_relu):
+        setattr_(fp8, f.__name__, f)
