@@ -67,9 +67,11 @@ class Encoder(_Layered):
             return eng.encode_layer(acts_norm, layer)
         return acts_norm @ self.W[layer] + self.b[layer]
 
-    def forward(self, acts_norm, layer="all"):
+    def forward(self, acts_norm, layer="all", eight_bit=False):
         if layer != "all":
             return self.forward_layer(acts_norm, layer)
+        if eight_bit:
+            return fp8.project(acts_norm, self.W, self.b)
         pre = torch.einsum("bld,ldf->blf", acts_norm, self.W).contiguous()
         return pre + self.b.to(acts_norm.dtype)
 
@@ -111,9 +113,11 @@ class Decoder(_Layered):
             features = features[:, :, layer, :]
         return features @ self.W[layer] + self.b[layer]
 
-    def forward(self, features, layer="all"):
+    def forward(self, features, layer="all", eight_bit=False):
         if layer != "all":
             return self.forward_layer(features, layer)
+        if eight_bit:
+            return fp8.project(features, self.W, self.b)
         return torch.einsum("blf,lfd->bld", features, self.W) + self.b
 
     def fold(self, output_standardizer: Standardizer):
@@ -153,9 +157,11 @@ class CrosslayerDecoder(_Layered):
             return eng.decode_layer(features, layer)
         return torch.einsum("bqsf,sfd->bqd", features, self.get_parameter(f"W_{layer}")) + self.b[layer]
 
-    def forward(self, features, layer="all"):
+    def forward(self, features, layer="all", eight_bit=False):
         if layer != "all":
             return self.forward_layer(features, layer)
+        if eight_bit:
+            return fp8.crosslayer_decode(features, self.blocks(), self.b)
         cols = [torch.einsum("bsf,sfd->bd", features[:, : t + 1], w).to(features.dtype)
                 for t, w in enumerate(self.blocks())]
         return torch.stack(cols, dim=1) + self.b.to(features.dtype)
@@ -167,6 +173,24 @@ class CrosslayerDecoder(_Layered):
                 w.data = w * output_standardizer.std[t]
             self._is_folded = True
         return self
+
+
+#: forwards that take ``eight_bit``
+_EIGHT_BIT = {cls.forward for cls in (Encoder, Decoder, CrosslayerDecoder, JumpReLU, ReLU)}
+
+
+def _run_eight_bit(module, x):
+    forward = module.__dict__.get("forward", type(module).forward)
+    if forward in _EIGHT_BIT:
+        return module(x, eight_bit=True)
+    if forward is nn.ReLU.forward and not module.inplace and not _has_hooks(module):
+        return fp8.jump_relu(x)             # (torch's class has no such argument)
+    return module(x)
+
+
+def _has_hooks(module):
+    return bool(module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks or module._backward_hooks
+                or nn.modules.module._has_any_global_hook())
 
 
 class CrossLayerTranscoder(SerializableModule):
@@ -208,25 +232,16 @@ class CrossLayerTranscoder(SerializableModule):
         return pre_actvs, features, recons_norm, recons
 
     def _forward_eight_bit(self, acts):
-        """The three products of ``forward`` through ``crosslayer_transcoder_b200.fp8``, results in the type of ``acts``.  Nonlinearities
-        other than (Jump)ReLU are the module's own.  A feature shard (``parallel.attach``) is refused: its features give a part of
+        """``forward`` up to the reconstructions, on 8-bit operands (``crosslayer_transcoder_b200.fp8``), results in the type of
+        ``acts``.  Every module is called as such, so that its hooks run; those with a forward of their own, other nonlinearities
+        than (Jump)ReLU among them, run that.  A feature shard (``parallel.attach``) is refused: its features give a part of
         the sum over all shards, and a TopK would select within the shard."""
-        enc, dec, nl = self.encoder, self.decoder, self.nonlinearity
-        engine = enc.__dict__.get("_kernel_engine")
+        engine = self.encoder.__dict__.get("_kernel_engine")
         if engine is not None and getattr(engine.module, "tp_world", 1) > 1:
             raise NotImplementedError("eight_bit runs on whole modules only, not on feature shards")
-        pre_actvs = fp8.project(acts, enc.W, enc.b)
-        if isinstance(nl, JumpReLU):
-            features = fp8.jump_relu(pre_actvs, nl.theta, nl.bandwidth)
-        elif isinstance(nl, (ReLU, nn.ReLU)):
-            features = fp8.jump_relu(pre_actvs)
-        else:
-            features = nl(pre_actvs)
-        if dec.crosslayer:
-            recons_norm = fp8.crosslayer_decode(features, dec.blocks(), dec.b)
-        else:
-            recons_norm = fp8.project(features, dec.W, dec.b)
-        return pre_actvs, features, recons_norm
+        pre_actvs = _run_eight_bit(self.encoder, acts)
+        features = _run_eight_bit(self.nonlinearity, pre_actvs)
+        return pre_actvs, features, _run_eight_bit(self.decoder, features)
 
     def _init_args(self):
         sub = lambda m: None if m is None else m.to_config()

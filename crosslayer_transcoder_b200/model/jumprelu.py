@@ -2,19 +2,21 @@
 
 In the training step both run fused into the encoder contraction's epilogue
 (forward) and into the feature-gradient contraction's epilogue (backward); the
-autograd function below is the eager definition for direct calls.
+autograd function below is the eager definition for direct calls.  With ``eight_bit`` a
+forward keeps two bits an element for backward (``crosslayer_transcoder_b200.fp8``).
 """
 from __future__ import annotations
 
 import torch
 from torch import nn
 
+from .. import fp8
 from .serializable_module import SerializableModule
 
 
 class ReLU(SerializableModule):
-    def forward(self, input, layer=None):
-        return torch.relu(input)
+    def forward(self, input, layer=None, eight_bit=False):
+        return fp8.jump_relu(input) if eight_bit else torch.relu(input)
 
 
 class _JumpReLUEager(torch.autograd.Function):
@@ -43,7 +45,9 @@ class JumpReLU(SerializableModule):
         self.register_buffer("bandwidth", torch.tensor(float(bandwidth)))
         self._init_theta, self.n_layers, self.d_features = theta, n_layers, d_features
 
-    def forward(self, input):
+    def forward(self, input, eight_bit=False):
+        if eight_bit:
+            return fp8.jump_relu(input, self.theta, self.bandwidth)
         return _JumpReLUEager.apply(input, self.theta, self.bandwidth)
 
     def _init_args(self):
