@@ -47,7 +47,10 @@ class JumpReLU(SerializableModule):
 
     def forward(self, input, eight_bit=False):
         if eight_bit:
-            return fp8.jump_relu(input, self.theta, self.bandwidth)
+            theta, shape = self.theta, input.shape[-2:]
+            if theta.shape[1:] != shape and all(a in (1, b) for a, b in zip(theta.shape[1:], shape)):
+                theta = theta.expand(1, *shape)         # one for all layers or features
+            return fp8.jump_relu(input, theta, self.bandwidth)
         return _JumpReLUEager.apply(input, self.theta, self.bandwidth)
 
     def _init_args(self):

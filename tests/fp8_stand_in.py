@@ -19,7 +19,8 @@ def jump_relu(x, theta=None, bandwidth=1.0):
     if theta is None:
         return torch.relu(x)
     inner = theta.shape[1:] if theta.shape[0] == 1 else theta.shape
-    assert x.shape[x.dim() - len(inner):] == inner
+    if x.shape[x.dim() - len(inner):] != inner:
+        raise ValueError(f"theta {tuple(theta.shape)} does not match the last axes of x {tuple(x.shape)}")
     return x * ((x > theta) & (x > 0))
 
 

@@ -130,3 +130,39 @@ def test_own_forwards_reach_the_operators(monkeypatch):
             calls.clear()
             model(x)
             assert calls == want.split()
+
+
+@pytest.mark.parametrize("layers, features", [(1, 1), (1, F), (L, 1), (L, F)])
+@pytest.mark.parametrize("batch", [1, B])
+def test_thresholds_that_broadcast(layers, features, batch):
+    """One threshold for all layers or features, as the eager definition takes it: same results, gradients in theta's shape."""
+    model = _model(JumpReLU(0.03, 1.0, layers, features))
+    x = torch.randn(batch, L, D)
+    eager, switched = _both(model, x)
+    assert all(torch.equal(a, b) for a, b in zip(eager, switched))
+    theta = model.nonlinearity.theta
+    if theta.shape[1:] != (L, F):
+        seen = []
+        theta.register_hook(lambda g: seen.append(g.shape))
+        pre = torch.randn(batch, L, F)
+
+        class Keep(torch.autograd.Function):                # thresholds as the operator gets them
+            @staticmethod
+            def forward(ctx, x, th):
+                assert th.shape == (1, L, F)
+                return x * (x > th)
+
+            @staticmethod
+            def backward(ctx, g):
+                return g, torch.ones(1, L, F)
+
+        from crosslayer_transcoder_b200 import fp8
+
+        fp8.jump_relu = lambda x, th, bw: Keep.apply(x, th)  # (put back with the fixture)
+        model.nonlinearity(pre, eight_bit=True).sum().backward()
+        assert torch.equal(theta.grad, torch.ones(1, L, F).sum_to_size(theta.shape)) and seen == [theta.shape]
+
+
+def test_thresholds_that_do_not_fit_are_refused():
+    with pytest.raises(ValueError):
+        JumpReLU(0.03, 1.0, L + 1, F)(torch.randn(B, L, F), eight_bit=True)
