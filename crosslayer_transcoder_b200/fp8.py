@@ -317,11 +317,12 @@ def _rows_first(x):
     return x, x.stride(0), x.stride(1)
 
 
-def _pass_forward(crosslayer, x, W, blocks, w_dtype, b, N):
-    """y [B, L, N] and the 8-bit copies of x [B, L, K] and of the weights (``W``, or the addresses of a decoder's ``blocks``)."""
+def _pass_forward(crosslayer, x, W, blocks, w_dtype, b, shape):
+    """y [B, L, N] as ``shape`` and the 8-bit copies of x [B, L, K] and of the weights (``W``, or the addresses of a decoder's
+    ``blocks``).  (y is made in its final shape: of a view that a node returns autograd refuses changes in place.)"""
     status, call, query, dev = _status_word(), lib().call, lib().query, x.device
-    B, L, K = x.shape
-    y = torch.empty(B, L, N, dtype=x.dtype, device=dev)
+    (B, L, K), N = x.shape, shape[-1]
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
     x_copy = torch.empty(256 * query("clt_fp8_copy_units", L, B, K), device=dev, **_BYTES)
     w_copy = torch.empty(256 * query("clt_fp8_copy_units", _pairs(L) if crosslayer else L, K, N), device=dev, **_BYTES)
     if B:
@@ -370,10 +371,10 @@ class _Project(torch.autograd.Function):
             x = x.reshape(xs.numel() // (L * K), L, K)
         if not W.is_contiguous():
             W = W.contiguous()
-        y, x_copy, w_copy = _on(x.device, _pass_forward, 0, x, W, None, W.dtype, b, N)
+        y, x_copy, w_copy = _on(x.device, _pass_forward, 0, x, W, None, W.dtype, b, (*xs[:-1], N))
         ctx.dims = x.shape[0], L, K, N
         ctx.save_for_backward(x_copy if need_w else None, w_copy if need_x else None)
-        return y if len(xs) == 3 and len(ws) == 3 else y.view(*xs[:-1], N)
+        return y
 
     @staticmethod
     @_first_order
@@ -429,10 +430,10 @@ class _CrosslayerDecode(torch.autograd.Function):
             dtype = torch.float32
             blocks = [w.float().contiguous() for w in blocks]
         at = array("Q", [w.data_ptr() for w in blocks])
-        y, f_copy, w_copy = _on(f.device, _pass_forward, 1, f, None, at.buffer_info()[0], dtype, b, D)
+        y, f_copy, w_copy = _on(f.device, _pass_forward, 1, f, None, at.buffer_info()[0], dtype, b, (*shape[:-1], D))
         ctx.dims = f.shape[0], L, F, D
         ctx.save_for_backward(f_copy if need_w else None, w_copy if ctx.needs_input_grad[0] else None)
-        return y if len(shape) == 3 else y.view(*shape[:-1], D)
+        return y
 
     @staticmethod
     @_first_order
