@@ -78,6 +78,7 @@ struct alignas(16) ScaleRing {
   float bias[kSlots][kBN];  // of tiles, which have a window each at least
   int4 tile[kSlots];  // with a tile's first window: row, column, output slab, blocks (0: there are no more tiles)
   uint32_t starts[kSlots];
+  uint32_t far[kSlots][2];  // some scale that a scale warp brought with the window is far_from_one
   uint64_t full[kSlots], empty[kSlots];
 };
 constexpr int kSmemBytes =
@@ -203,6 +204,28 @@ __device__ __forceinline__ void fma16(float* acc, const uint32_t (&d)[16], float
 #pragma unroll
   for (int i = 0; i < 16; ++i) acc[i] = fmaf(__uint_as_float(d[i]), s, acc[i]);
 }
+__device__ __forceinline__ void mul16(uint32_t (&d)[16], float s) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) d[i] = __float_as_uint(__uint_as_float(d[i]) * s);
+}
+// Scales whose product with another may not be one of fp32's normal numbers: below 2^-63 or from 2^63 on (zeros, infinities and NaN
+// among them).
+__device__ __forceinline__ bool far_from_one(float s) {
+  return (__float_as_uint(s) & 0x7fffffffu) - (64u << 23) >= 126u << 23;
+}
+// One is then applied after the other where their product is not normal.  A sum d of products is 0 or 2^-18 to 2^28 in magnitude.  Of
+// a small product the larger scale comes first (below 2^23: the other is at least 2^-149), of a large one the smaller (above 1), so
+// that d times it neither overflows nor loses bits unless the result does.
+struct Factors {
+  float first, second;
+  __device__ __forceinline__ Factors(float a, float b) {
+    first = 1.f, second = a * b;
+    if (!(fabsf(second) >= 0x1p-126f && fabsf(second) <= 3.402823466e38f) && a != 0.f && b != 0.f) {
+      const bool a_first = fabsf(second) < 1.f ? fabsf(a) > fabsf(b) : fabsf(a) < fabsf(b);
+      first = a_first ? a : b, second = a_first ? b : a;
+    }
+  }
+};
 
 // ---- stores -------------------------------------------------------------------------------------
 template <class T>
@@ -534,13 +557,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
                 pa0 += sa.k, pa1 += sa.k, pb += sb.k, --seg_left;
               }
             }
+            bool far = false;
 #pragma unroll
             for (int i = 0; i < window; ++i) {
               if (i < n) {
                 ring->a[slot][i * 128 + t] = va[i], ring->a[slot][i * 128 + t + 64] = vb[i];
-                if (t < 2) ring->b[slot][i][t] = vc[i];
+                far |= far_from_one(va[i]) || far_from_one(vb[i]);
+                if (t < 2) ring->b[slot][i][t] = vc[i], far |= far_from_one(vc[i]);
               }
             }
+            far = __any_sync(0xffffffffu, far);
+            if (lane == 0) ring->far[slot][warp - 2] = far;
           } else if (warp == 2) {
             // lane i has block at + i: its scales of both CTAs' rows and of both halves of the columns
             float v[4] = {};
@@ -553,7 +580,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
               v[2] = __ldg(b0 + zb * sb.z + kb * sb.k);
               v[3] = __ldg(b1 + zb * sb.z + kb * sb.k);
             }
-            bool differs = lane == 0;
+            bool differs = lane == 0, far = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) far |= lane < n && far_from_one(v[i]);
+            far = __any_sync(0xffffffffu, far);
 #pragma unroll
             for (int i = 0; i < 4; ++i) differs |= !(v[i] == __shfl_up_sync(0xffffffffu, v[i], 1));
             const uint32_t changes = __ballot_sync(0xffffffffu, differs && lane < n);
@@ -569,7 +599,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
               ring->a[slot][group] = rank == 0 ? v[0] : v[1];
               ring->b[slot][group][0] = v[2], ring->b[slot][group][1] = v[3];
             }
-            if (lane == 0) ring->starts[slot] = starts;
+            if (lane == 0) ring->starts[slot] = starts, ring->far[slot][0] = far, ring->far[slot][1] = 0;
           }
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->full[slot]));
@@ -628,39 +658,56 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant_
         if (left < tile.w) alive = window_ready(batch);
         const float* ra = ring->a[slot] + (kByRow ? quarter * 32 + lane : 0);
         const float* rb = &ring->b[slot][0][half];
+        const bool far = (ring->far[slot][0] | ring->far[slot][1]) != 0;
         const int groups = kByRow ? min(left, window) : __popc(ring->starts[slot]);
+        // Where the scale warps found a scale far from one, one scale is applied after the other (Factors).  That is a loop of its
+        // own: 12 x 4000 x 768 x 24576 by rows 1193 us (1174 without such scales being provided for; 1556 where all are such),
+        // 1216 with a look at every product inside one loop, 1236 with the flag there.
+        const auto blocks = [&](auto kind) {
+          constexpr bool split = decltype(kind)::value;
 #pragma unroll 1
-        for (int i = 0; alive && i < groups; ++i, ++n) {
-          const float s = ra[kByRow ? i * 128 : i] * rb[i * 2];
-          const int buf = n & 1;
-          const uint32_t taddr = tbase + buf * kBN;
-          if (work) {
+          for (int i = 0; alive && i < groups; ++i, ++n) {
+            float s = ra[kByRow ? i * 128 : i] * rb[i * 2], first = 1.f;
+            if constexpr (split) {
+              const Factors f(ra[kByRow ? i * 128 : i], rb[i * 2]);
+              first = f.first, s = f.second;
+            }
+            const int buf = n & 1;
+            const uint32_t taddr = tbase + buf * kBN;
+            if (work) {
 #pragma unroll
-            for (int c = 0; c < 8; c += 2) {
-              tmem_ld_wait(r0);
-              tmem_ld16_issue(taddr + 16 * (c + 1), r1);
-              fma16(acc + 16 * c, r0, s);
-              tmem_ld_wait(r1);
-              if (c < 6) {
-                tmem_ld16_issue(taddr + 16 * (c + 2), r0);
-                fma16(acc + 16 * (c + 1), r1, s);
+              for (int c = 0; c < 8; c += 2) {
+                tmem_ld_wait(r0);
+                tmem_ld16_issue(taddr + 16 * (c + 1), r1);
+                if constexpr (split) mul16(r0, first);
+                fma16(acc + 16 * c, r0, s);
+                tmem_ld_wait(r1);
+                if constexpr (split) mul16(r1, first);
+                if (c < 6) {
+                  tmem_ld16_issue(taddr + 16 * (c + 2), r0);
+                  fma16(acc + 16 * (c + 1), r1, s);
+                }
               }
             }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (kPair)
+                arrive_remote(tc::cluster_addr(tc::smem_u32(&bars->tmem_empty[buf]), 0));
+              else
+                tc::mbar_arrive(tc::smem_u32(&bars->tmem_empty[buf]));
+            }
+            if (i + 1 < groups || left > window) {
+              alive = block_ready(bars, n + 1, abort_flag, status);
+              if (alive && work) tmem_ld16_issue(tbase + ((n + 1) & 1) * kBN, r0);
+            }
+            if (work) fma16(acc + 112, r1, s);
           }
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (kPair)
-              arrive_remote(tc::cluster_addr(tc::smem_u32(&bars->tmem_empty[buf]), 0));
-            else
-              tc::mbar_arrive(tc::smem_u32(&bars->tmem_empty[buf]));
-          }
-          if (i + 1 < groups || left > window) {
-            alive = block_ready(bars, n + 1, abort_flag, status);
-            if (alive && work) tmem_ld16_issue(tbase + ((n + 1) & 1) * kBN, r0);
-          }
-          if (work) fma16(acc + 112, r1, s);
-        }
+        };
+        if (far)
+          blocks(std::true_type());
+        else
+          blocks(std::false_type());
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_u32(&ring->empty[slot]));
         if (left <= window && alive && work) store_warp<kOut>(acc, buf8, &mapOut, out, zo, row0, col0, g.M, g.N);

@@ -280,8 +280,7 @@ def matmul(a: BlockTensor, b: BlockTensor, bias: Optional[torch.Tensor] = None,
            out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a [M, K] @ b [K, N] (+ bias [N])``, or stacks ``[Z, M, K] @ [Z, K, N] (+ bias [N] or [Z, N])``, in fp32 sums that are
     rounded once to ``out_dtype``.  ``a`` has blocks of 1 x 128 or 128 x 128 (with 1 x 128 only untransposed: its blocks have to
-    lie along the contraction), ``b`` blocks of 128 x 128; either may be a transposed view (``.mT``).  The products of the
-    operands' scales have to be finite.  Values whose rows do not start on 16 bytes are copied first."""
+    lie along the contraction), ``b`` blocks of 128 x 128; either may be a transposed view (``.mT``).  Values whose rows do not start on 16 bytes are copied first."""
     if not isinstance(a, BlockTensor) or not isinstance(b, BlockTensor):
         raise TypeError(f"a and b must be BlockTensors, got {type(a).__name__} and {type(b).__name__}")
     sa, sb = a.shape, b.shape

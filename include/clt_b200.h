@@ -503,7 +503,7 @@ int clt_fp8_dequantize(const void* q, int64_t q_ld, int64_t q_z, const float* sc
 int clt_fp8_align(const void* q, int64_t q_ld, int64_t q_z, void* out, int64_t pitch, int Z, int R, int C, clt_stream_t stream);
 /* out[z] = A B + bias[z] over slabs z, in fp32 sums, rounded once to out_dtype.  A [M, K] (a_trans: stored [K, M]) with blocks of
  * a_rows x 128 (a_trans: 128 x 128), B [K, N] (b_trans: stored [N, K]) with blocks of 128 x 128; a_mn / a_k: distances of the
- * scales between blocks along M and along K, likewise for B along N and K.  Any fp32 scales will do whose products are finite.
+ * scales between blocks along M and along K, likewise for B along N and K.  Any fp32 scales will do.
  *   mode 0: L slabs, A and B stacked [L]
  *   mode 1: slab t of L sums A[s] B[pair(t, s)] over s <= t (crosslayer decoder)
  *   mode 2: slab s of L sums A[t] B[pair(t, s)] over t >= s (its feature gradient)

@@ -1,10 +1,12 @@
-"""Calls of the 8-bit operators at the ends of what they take: thresholds that broadcast, scales that are no powers of two."""
+"""Calls of the 8-bit operators at the ends of what they take: thresholds that broadcast, scales that are no powers of two,
+scales whose products fp32 does not hold."""
 import numpy as np
 import pytest
 import torch
 
 from crosslayer_transcoder_b200 import fp8
 from crosslayer_transcoder_b200.model import JumpReLU
+from tests import fp8_reference as ref
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -82,3 +84,83 @@ def test_read_back_is_rounded_once(dtype, columns):
         want = once(codes.double()[None] * scales.double().repeat_interleave(128, 1)[:, :columns], dtype)
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+# ---- products of scales outside of fp32's normal numbers -----------------------------------------------------------------------
+def _scales(shape, low, high, g):
+    """Numbers of any mantissa with exponents from `low` to `high`."""
+    return ((1 + torch.rand(shape, generator=g).double()) * 2.0 ** torch.randint(low, high + 1, shape, generator=g)).float()
+
+
+def _far_operands(kind, M, K, N, rows, a_t, b_t, g):
+    kb = -(-K // 128)
+    va, vb = torch.randn(M, K, generator=g), torch.randn(K, N, generator=g)
+    sa, sb = (-(-M // rows), kb), (kb, -(-N // 128))
+    if kind == "small":                                         # products of 2^-156 to 2^-134
+        va, vb = va * 100, vb * 100
+        sa, sb = _scales(sa, -106, -94, g), _scales(sb, -50, -40, g)
+    else:                                                       # of 2^128 to 2^134, and values of 2^-9 or 0
+        va, vb = va.sign() * (va.abs() > 1) * 2.0 ** -9, vb.sign() * (vb.abs() > 1) * 2.0 ** -9
+        sa, sb = _scales(sa, 60, 62, g), _scales(sb, 68, 70, g)
+    zero = slice(M // 2, M // 2 + (M > 1))
+    va[zero] = 0                                                # a row of zeros
+    va, vb = va.clamp(-448, 448).to(torch.float8_e4m3fn), vb.clamp(-448, 448).to(torch.float8_e4m3fn)
+    da = va.double() * sa.double().repeat_interleave(rows, 0)[:M].repeat_interleave(128, 1)[:, :K]
+    db = vb.double() * sb.double().repeat_interleave(128, 0)[:K].repeat_interleave(128, 1)[:, :N]
+    t = lambda v, s, r, turned: (fp8.BlockTensor(v.t().contiguous().to(DEV), s.t().contiguous().to(DEV), r).mT if turned else
+                                 fp8.BlockTensor(v.to(DEV), s.to(DEV), r))
+    return t(va, sa, rows, a_t), t(vb, sb, 128, b_t), da, db, zero
+
+
+@pytest.mark.parametrize("layout", [(1, False, False), (128, False, False), (1, False, True), (128, True, False), (128, True, True)])
+@pytest.mark.parametrize("shape", [(70, 300, 140), (1, 5000, 72), (2500, 640, 2600), (257, 1024, 33)])
+@pytest.mark.parametrize("kind", ["small", "large"])
+def test_scales_whose_product_fp32_does_not_hold(kind, shape, layout):
+    M, K, N = shape
+    a, b, da, db, zero = _far_operands(kind, M, K, N, *layout, torch.Generator().manual_seed(11))
+    want, mags = da @ db, da.abs() @ db.abs()
+    assert float(mags.max()) < 2.0 ** 127 and float(mags.max()) > 2.0 ** -126      # results are numbers of fp32
+    for out in (torch.float32, torch.bfloat16):
+        y = fp8.matmul(a, b, out_dtype=out)
+        # below 2^-126 each addition (one a block, and one a part) and the last rounding are off by half of the least number
+        least = 2.0 ** -149 if out == torch.float32 else 2.0 ** -133
+        ref.check(y, want, mags, K, extra=(-(-K // 128) * 2 + 2) * 2.0 ** -150 + least / 2)
+        assert not y[zero].any()
+    fp8.check_status()
+
+
+def test_rows_of_small_ordinary_and_large_scales():
+    """Side by side in a warp; zero, infinite and NaN scales reach their own rows alone."""
+    M, K, N = 96, 384, 260
+    g = torch.Generator().manual_seed(12)
+    va = (torch.randn(M, K, generator=g).sign() * 2.0 ** -9).to(torch.float8_e4m3fn)
+    vb = (torch.randn(K, N, generator=g).sign() * 2.0 ** -9).to(torch.float8_e4m3fn)
+    sb = torch.full((3, 3), 1.5 * 2.0 ** 20)
+    sa = torch.tensor([2.0 ** -149, 1.1 * 2.0 ** -147, 1.7 * 2.0 ** 115, 1.0, 0.0, 2.0 ** 108, 3.0, 1.3 * 2.0 ** -146])[:, None].repeat(12, 3)
+    sa[17, 1], sa[40, 2] = float("inf"), float("nan")
+    y = fp8.matmul(fp8.BlockTensor(va.to(DEV), sa.to(DEV), 1), fp8.BlockTensor(vb.to(DEV), sb.to(DEV)), out_dtype=torch.float32).cpu()
+    bad = torch.zeros(M, dtype=torch.bool)
+    bad[17] = bad[40] = True
+    da, db = va.double() * sa.double().repeat_interleave(128, 1), vb.double() * sb.double().repeat_interleave(128, 0)[:, :1]
+    ref.check(y[~bad], da[~bad] @ db, da[~bad].abs() @ db.abs(), K, extra=10 * 2.0 ** -149)
+    assert not y[4::8].any() and not y[bad].isfinite().any()
+
+
+@pytest.mark.parametrize("large", [False, True])
+def test_passes_of_small_and_large_numbers(large):
+    """Blocks whose scales have a product of 2^-152, or of 2^129 (from one row and one column), and results that are numbers of fp32."""
+    B, D, F = 40, 2001, 72
+    g = torch.Generator().manual_seed(13)
+    x, W = torch.rand(B, 1, D, generator=g) * 0.5 + 0.5, torch.rand(1, D, F, generator=g) * 0.5 + 0.5
+    x, W = (x * 2.0 ** 112, W * 2.0 ** 3) if large else (x * 2.0 ** -80, W * 2.0 ** -56)
+    x[0] = 0
+    if large:
+        x[1], W[:, :, 0] = 2.0 ** 127, 2.0 ** 18
+    y = fp8.project(x.to(DEV), W.to(DEV)).cpu()
+    xq, wq = ref.rounded(x.transpose(0, 1)), ref.rounded(W)
+    want = (xq @ wq).transpose(0, 1)
+    fits = want < 2.0 ** 127.9
+    assert float(fits.double().mean()) > 0.9 and float(want[fits].max()) > 2.0 ** -126
+    at = lambda t: torch.where(fits, t, torch.zeros_like(t))
+    ref.check(at(y), at(want), at(want), D, extra=40 * 2.0 ** -150)
+    assert not y[0].any()
