@@ -529,15 +529,14 @@ class _JumpReLU(torch.autograd.Function):
                 value = float(bandwidth)
         y, bits = _on(x.device, _jump_relu_forward, x, C, th, bw, value)
         ctx.value, ctx.C = value, C
-        ctx.save_for_backward(bits, theta, bw)
+        # (where the gradient passes, the bits say by themselves)
+        ctx.save_for_backward(bits, *((theta, bw) if ctx.needs_input_grad[1] else (None, None)))
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, g):
         bits, theta, bw = ctx.saved_tensors
-        if not ctx.needs_input_grad[1]:
-            theta = None                        # (where the gradient passes, the bits say by themselves)
         th = theta
         if th is not None and (th.dtype != torch.float32 or not th.is_contiguous()):
             th = th.float().contiguous()

@@ -48,3 +48,22 @@ def test_results_may_be_changed_in_place(call):
     assert y.shape == shape and y.shape[:-1] == leaves[0].shape[:-1] and y.is_contiguous()
     y.sum().backward()
     assert all(t.grad.shape == t.shape for t in leaves)
+
+
+def test_thresholds_without_a_gradient_are_not_kept():
+    """x's gradient takes the two bits alone: such thresholds and the bandwidth may change, or be inference tensors."""
+    with torch.inference_mode():
+        frozen = torch.zeros(7)
+    for theta in (torch.zeros(7), frozen):
+        x, bandwidth = torch.zeros(4, 7, requires_grad=True), torch.ones(())
+        y = fp8.jump_relu(x, theta, bandwidth)
+        if theta is not frozen:
+            theta.add_(1.0)
+        bandwidth.mul_(0.5)
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+    x, theta = torch.zeros(4, 7, requires_grad=True), torch.zeros(7, requires_grad=True)
+    y = fp8.jump_relu(x, theta, bandwidth)
+    bandwidth.mul_(0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):     # the thresholds' gradient does take it
+        y.sum().backward()
