@@ -6,8 +6,10 @@
 // one to e4m3 (half a step: 2^-4 of the value), whichever way a copy was made, and a copy of a copy is the copy.  e4m3 has no
 // infinity: what is not finite becomes NaN, and does not count for the scale.
 //
-// All kernels here are bound by memory: 12 x 4000 x 10000 bf16 to 8 bits 231 us (6.2 TB/s), back 226 (6.4); a gradient with its column
-// sums, 12 x 4000 x 24576, 573 (6.2); JumpReLU of that size 780 (6.4) and its backward 790 (6.3), ReLU 765 (6.5) and 723 (6.9).
+// Where rows start on 16 bytes the kernels are bound by memory: 12 x 4000 x 10000 bf16 to 8 bits 225 us (6.4 TB/s), by rows 245 (5.9),
+// back 226 (6.4); a gradient with its column sums, 12 x 4000 x 24576, 573 (6.2); JumpReLU of that size 780 (6.4) and its backward 790
+// (6.3), ReLU 765 (6.5) and 723 (6.9).  Other rows cost more instructions, which bound them: 6 x 4000 x 10001 bf16 to 8 bits 180 us,
+// by rows 162, back 214, where 10000 columns take 117, 125 and 116; JumpReLU 278 and 249 (166 and 185), ReLU 206 and 201 (163 and 154).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

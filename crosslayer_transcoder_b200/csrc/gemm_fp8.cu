@@ -17,10 +17,12 @@ bool use_pair(const GemmGeom& g, int sms) {
 }
 
 // Cuts the contraction into parts (gemm.cuh) where that is estimated faster; sets g.kb_per_part and returns the number of parts, or
-// 0 for whole chains.  Estimates, in us: 0.45 a block of 128 x 256 x 128 (a CTA's, or a pair's of 256 rows), 1.5 a tile for its
+// 0 for whole chains.  Estimates, in us: 0.45 a block of 128 x 256 x 128 (a CTA's, or a pair's of 256 rows; what joined blocks
+// take.  Separate ones take 0.60, which the plan does not know: it gets no scales), 1.5 a tile for its
 // output and the next one's start; partial sums go to memory and back at 5 TB/s, behind a launch of 4.  Parts are tried that
 // fill 1 to 8 rounds of the chip: 257 x 120000 x 768 in 17 parts of 58 blocks, 153 tiles, took 47 us, in 16 of 59, one
-// round, 42; whole chains 500.
+// round, 42 (the product by itself; the call 49 on the device with the parts' sum and the gap between the two launches); whole
+// chains 500.
 int plan_parts(GemmGeom& g, int sms) {
   const int kb_per_seg = (int)up(g.Kseg, f8::kBK);
   const bool pair = pair_rows(g.M);

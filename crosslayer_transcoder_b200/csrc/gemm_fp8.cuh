@@ -23,7 +23,7 @@
 //     32-wide K step of one MMA moves the start address by 4096 B (K-major: by 32 B).
 // What bounds it now: joined blocks, shared memory (stages written and read: 64 KB a block and SM) and, with few blocks to a tile,
 // the output's way to memory (12 x 4000 x 768 x 24576: 943 us, 740 without the copies); separate ones, the epilogue above, and for
-// few blocks its start and output between the tiles (1190 us; scales by row 1245).
+// few blocks its start and output between the tiles (1190 us; scales by row and a bias 1290).
 // Tried without gain: MMAs of half the columns, each half of the epilogue on its own two accumulators (925 -> 997 us); sixteen
 // epilogue warps of 64 columns (975); reads of 32 columns, packed FMAs, five stages, two stages to an MMA round.
 //
